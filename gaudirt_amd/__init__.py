@@ -114,7 +114,8 @@ def _call_directly(torch):
         Direct.__name__, Direct.__qualname__, Direct.__module__ = base.__name__, base.__qualname__, base.__module__
         return Direct
 
-    for name, position in (("paged_attn", 5), ("rotary_paged_attn", 6), ("rotary_embedding", 3)):
+    for name, position in (("paged_attn", 5), ("rotary_paged_attn", 6), ("rotary_embedding", 3),
+                           ("shared_prefix_attn", 5), ("paged_attn_alibi", 5)):
         packet = getattr(torch.ops.gaudirt, name)
         if callable(getattr(packet, "_op", None)):
             packet.__class__ = direct(type(packet), position)
@@ -171,6 +172,29 @@ def _register_fakes(torch):
         torch._check(key.shape[0] == query.shape[0])
         torch._check(value.shape[0] == query.shape[0])
         return torch.empty_like(query, memory_format=torch.contiguous_format)
+
+
+    @torch.library.register_fake("gaudirt::shared_prefix_attn")
+    def _fake_shared_prefix_attn(query, key, value, key_pool, value_pool, metadata, group_rows, group_prefix,
+                                 head_dim, scale, softcap=0.0, sliding_window=-1):
+        torch._check(key.shape[0] == query.shape[0])
+        torch._check(value.shape[0] == query.shape[0])
+        return torch.empty_like(query, memory_format=torch.contiguous_format)
+
+    @torch.library.register_fake("gaudirt::paged_attn_alibi")
+    def _fake_paged_attn_alibi(query, key, value, key_pool, value_pool, metadata, slopes, head_dim, scale,
+                               softcap=0.0, sliding_window=-1):
+        torch._check(key.shape[0] == query.shape[0])
+        torch._check(value.shape[0] == query.shape[0])
+        return torch.empty_like(query, memory_format=torch.contiguous_format)
+
+    @torch.library.register_fake("gaudirt::extend_block_tables")
+    def _fake_extend_block_tables(block_tables, mapping, requests, prefixes, lengths, free_pages, free_head, parents,
+                                  page_size, slots, max_rows):
+        torch._check(prefixes.shape[0] == requests.shape[0])
+        torch._check(lengths.shape[0] == requests.shape[0])
+        rows = [block_tables.new_empty([max_rows]) for _ in range(3)]
+        return (*rows, torch.empty_like(lengths, memory_format=torch.contiguous_format), block_tables.new_empty([4]))
 
 
 def allocate_paged_kv(layers, slots, kv_heads, head_dim):

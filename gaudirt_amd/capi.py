@@ -42,6 +42,9 @@ EXPORTED = [
     "gk_allocator_create", "gk_allocator_destroy", "gk_allocator_alloc", "gk_allocator_record_stream",
     "gk_allocator_free", "gk_allocator_empty_cache", "gk_allocator_get_stats",
     "gk_rotary_embedding", "gk_rotary_kv_store",
+    "gk_paged_decode_alibi_workspace_bytes", "gk_paged_decode_alibi", "gk_paged_prefill_alibi",
+    "gk_shared_prefix_list_build", "gk_shared_prefix_workspace_bytes", "gk_shared_prefix_attention",
+    "gk_extend_block_tables",
 ]
 
 c_void_p = ctypes.c_void_p
@@ -93,6 +96,33 @@ class PrefillList(_Sized):
         ("struct_size", ctypes.c_size_t),
         ("items", c_void_p), ("merges", c_void_p), ("row_request", c_void_p),
         ("item_count", c_i32), ("merge_count", c_i32), ("part_slots", c_i32),
+    ]
+
+
+class SharedPrefixList(_Sized):
+    _fields_ = [
+        ("struct_size", ctypes.c_size_t),
+        ("words", c_void_p), ("row_request", c_void_p),
+        ("part_cols", c_i64),
+        ("rows", c_i32), ("tile_count", c_i32), ("workers", c_i32), ("worker_groups", c_i32), ("word_count", c_i32),
+        ("map_at", c_i32), ("position_at", c_i32), ("merges_at", c_i32), ("tiles_at", c_i32), ("workers_at", c_i32),
+        ("segments_at", c_i32),
+    ]
+
+
+class ExtendParams(_Sized):
+    _fields_ = [
+        ("struct_size", ctypes.c_size_t),
+        ("block_tables", c_void_p), ("mapping", c_void_p),
+        ("requests", c_i32), ("pages", c_i32), ("context", c_i32),
+        ("seq_requests", c_void_p), ("prefixes", c_void_p), ("lengths", c_void_p), ("parents", c_void_p),
+        ("free_pages", c_void_p), ("free_head", c_void_p),
+        ("requests_int64", c_i32), ("lengths_int64", c_i32), ("pages_int64", c_i32),
+        ("free_count", c_i64),
+        ("batch", c_i32), ("page_size", c_i32),
+        ("slots", c_i64), ("max_rows", c_i32),
+        ("out_locations", c_void_p), ("out_requests", c_void_p), ("out_positions", c_void_p),
+        ("out_lengths", c_void_p), ("counts", c_void_p),
     ]
 
 
@@ -199,6 +229,18 @@ def load():
     lib.gk_allocator_get_stats.argtypes = [c_void_p, ctypes.POINTER(AllocatorStats)]
     lib.gk_rotary_embedding.argtypes = [ctypes.POINTER(RotaryParams), c_void_p]
     lib.gk_rotary_kv_store.argtypes = [ctypes.POINTER(RotaryParams), c_void_p]
+    lib.gk_paged_decode_alibi_workspace_bytes.restype = ctypes.c_size_t
+    lib.gk_paged_decode_alibi_workspace_bytes.argtypes = [ctypes.POINTER(DecodeParams)]
+    lib.gk_paged_decode_alibi.argtypes = [ctypes.POINTER(DecodeParams), c_void_p, c_void_p, ctypes.c_size_t, c_void_p]
+    lib.gk_paged_prefill_alibi.argtypes = [ctypes.POINTER(PrefillParams), ctypes.POINTER(PrefillList), c_void_p,
+                                           c_void_p, ctypes.c_size_t, c_void_p]
+    lib.gk_shared_prefix_list_build.argtypes = [c_void_p] * 4 + [c_i32, c_void_p] + [c_i32] * 5 + [
+        c_void_p, c_i64, ctypes.POINTER(SharedPrefixList)]
+    lib.gk_shared_prefix_workspace_bytes.restype = ctypes.c_size_t
+    lib.gk_shared_prefix_workspace_bytes.argtypes = [ctypes.POINTER(PrefillParams), ctypes.POINTER(SharedPrefixList)]
+    lib.gk_shared_prefix_attention.argtypes = [ctypes.POINTER(PrefillParams), ctypes.POINTER(SharedPrefixList),
+                                               c_void_p, ctypes.c_size_t, c_void_p]
+    lib.gk_extend_block_tables.argtypes = [ctypes.POINTER(ExtendParams), c_void_p]
     _lib = lib
     return lib
 

@@ -38,6 +38,7 @@ struct DecodeArgs {
   float* part_o;
   float* part_ml;
   uint16_t* pool_out;  // the pool as a store target (decode_unit.hip)
+  const float* slopes; // [q_heads] distance slopes (kScoreBias)
 };
 
 template <int D>
@@ -75,15 +76,15 @@ constexpr int unit_max_keys(int head_dim) { return head_dim == 64 ? 3072 : (1 <<
 constexpr int unit_short_keys(int waves) { return 128 * waves; }  // with fewer than eight waves
 constexpr int kUnitMaxNewRows = 256;
 bool unit_decode_fits(const gk_decode_params* params, int64_t units);
-int launch_unit_decode(const DecodeArgs& a, bool softcap, int head_dim, const gk_decode_params* params, bool store,
+int launch_unit_decode(const DecodeArgs& a, int score, int head_dim, const gk_decode_params* params, bool store,
                        hipStream_t stream);
 
 // Balanced ("stream") decode schedule, head dims 64/128/256, GQA group >= 4,
 // any block size. Workspace layout: part_o[2 * wgs][hpw][D],
 // part_ml[2 * wgs][hpw][2] and unit_span[units] (int32 pairs).
-int stream_decode_wgs(int head_dim, bool softcap, int block_size);
+int stream_decode_wgs(int head_dim, int score, int block_size);
 size_t stream_decode_workspace_bytes(int head_dim, int heads_per_group, int64_t units, int wgs);
-int launch_stream_decode(const DecodeArgs& a, bool softcap, int head_dim, int wgs, void* workspace,
+int launch_stream_decode(const DecodeArgs& a, int score, int head_dim, int wgs, void* workspace,
                          hipStream_t stream);
 
 }  // namespace gk

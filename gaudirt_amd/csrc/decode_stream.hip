@@ -139,11 +139,13 @@ constexpr int kTileBlocks = 0, kLoadBlocks = 1, kKeyBlocks = 2;
 constexpr int kArithMfma = 0, kArithDot = 1;
 constexpr int kDotMaxHeads = 3;
 
-template <int D, bool SOFTCAP, int MODE, int ARITH>
+template <int D, int SCORE, int MODE, int ARITH>
 __device__ __forceinline__ void decode_stream_body(StreamArgs sa) {
   using S = MfmaShape<D>;
+  constexpr bool LOG2 = SCORE != kScorePlain;  // scores in log2 units before the maxima, not raw products
   constexpr int TS = S::TS;
   constexpr bool DOT = ARITH == kArithDot;
+  static_assert(!DOT || SCORE != kScoreBias, "the dot form has no distance bias");
   static_assert(!DOT || TS == 32, "the dot form pairs each key with two lanes (head_dim 64/128)");
   constexpr int DNC = D / 16;  // dot form: 16-byte chunks of a key row per lane (half the row)
   constexpr int DOD = D / 64;  // dot form: output dims per lane
@@ -438,6 +440,7 @@ __device__ __forceinline__ void decode_stream_body(StreamArgs sa) {
   // threshold of a re-base; and the base of the probabilities (m_run, or 0
   // before the first maximum). Both change only at a re-base.
   float m_thr = -INFINITY, m_base = 0.f;
+  [[maybe_unused]] float slope = 0.f;  // the unit's distance slope of head c16
   const float inv_scale = 1.f / a.score_scale;
 
   // Maximum and sum over the 32 keys of a tile in the dot form (lanes l and
@@ -654,9 +657,9 @@ __device__ __forceinline__ void decode_stream_body(StreamArgs sa) {
       const float part = a0 + a1;
       const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(part), __float_as_uint(part), false, false);
       float sv = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-      if constexpr (SOFTCAP) sv = soft_cap(sv * a.score_scale, a.softcap_log2);
+      if constexpr (LOG2) sv = soft_cap(sv * a.score_scale, a.softcap_log2);
       const int k = t.tb + key;
-      sd[h] = (SOFTCAP || !(t.tb >= t.left && t.tb + TS <= t.ctx)) ? ((k >= t.left && k < t.ctx) ? sv : -INFINITY)
+      sd[h] = (LOG2 || !(t.tb >= t.left && t.tb + TS <= t.ctx)) ? ((k >= t.left && k < t.ctx) ? sv : -INFINITY)
                                                                     : sv;
     }
     // Re-base each head whose tile maximum passes its threshold.
@@ -665,13 +668,13 @@ __device__ __forceinline__ void decode_stream_body(StreamArgs sa) {
 #pragma unroll
     for (int h = 0; h < kDotMaxHeads; ++h) {
       mx[h] = h < hv ? key32_max(sd[h]) : -INFINITY;
-      any = any || mx[h] > (SOFTCAP ? dm_run[h] + kDecodeRescaleSlack : dm_thr[h]);
+      any = any || mx[h] > (LOG2 ? dm_run[h] + kDecodeRescaleSlack : dm_thr[h]);
     }
     if (__builtin_amdgcn_ballot_w64(any)) {
 #pragma unroll
       for (int h = 0; h < kDotMaxHeads; ++h) {
-        if (!(mx[h] > (SOFTCAP ? dm_run[h] + kDecodeRescaleSlack : dm_thr[h]))) continue;  // uniform
-        const float m_new = fmaxf(dm_run[h], SOFTCAP ? mx[h] : mx[h] * a.score_scale);
+        if (!(mx[h] > (LOG2 ? dm_run[h] + kDecodeRescaleSlack : dm_thr[h]))) continue;  // uniform
+        const float m_new = fmaxf(dm_run[h], LOG2 ? mx[h] : mx[h] * a.score_scale);
         const float alpha = dm_run[h] == -INFINITY ? 0.f : fast_exp2(dm_run[h] - m_new);
         dl[h] *= alpha;
 #pragma unroll
@@ -686,7 +689,7 @@ __device__ __forceinline__ void decode_stream_body(StreamArgs sa) {
     uint32_t pp[kDotMaxHeads];
 #pragma unroll
     for (int h = 0; h < kDotMaxHeads; ++h) {
-      const float p = SOFTCAP ? fast_exp2(sd[h] - dm_base[h]) : fast_exp2(__builtin_fmaf(sd[h], a.score_scale, -dm_base[h]));
+      const float p = LOG2 ? fast_exp2(sd[h] - dm_base[h]) : fast_exp2(__builtin_fmaf(sd[h], a.score_scale, -dm_base[h]));
       dl[h] += h < hv ? p : 0.f;
       const uint32_t b = bf16_bits(p);
       const uint32_t nb = __float_as_uint(dpp<kDppQuadXor1>(__uint_as_float(b)));
@@ -737,6 +740,10 @@ __device__ __forceinline__ void decode_stream_body(StreamArgs sa) {
         l_run = 0.f;
         m_thr = -INFINITY;
         m_base = 0.f;
+        if constexpr (SCORE == kScoreBias) {
+          const int kvh = kv_head_of(t), hg = t.h - kvh * a.head_groups;
+          slope = column_slope(a.slopes, kvh * a.group + hg * 16, min(16, a.group - hg * 16), c16);
+        }
       }
     }
     if constexpr (DOT) {
@@ -764,20 +771,22 @@ __device__ __forceinline__ void decode_stream_body(StreamArgs sa) {
       for (int c = 0; c < S::NC; ++c) sc[h] = mfma32(kr[h][c], qb[c], sc[h]);
     }
 
-    if constexpr (!SOFTCAP) mfma_results_ready(sc);
+    if constexpr (!LOG2) mfma_results_ready(sc);
+    if constexpr (SCORE == kScoreBias)
+      bias_scores(sc, a.score_scale, a.softcap_log2, slope, (float)(t.tb + 4 * q - t.ctx + 1));
 
     // Mask, and the row maximum over this lane's scores. Without softcap the
     // scores stay raw: a tile whose keys are all visible needs no per-element
     // mask, the maximum is compared with (m_run + kDecodeRescaleSlack) / scale
     // (kept with m_run), and the scale folds into the exponent below.
-    const bool inside = !SOFTCAP && t.tb >= t.left && t.tb + TS <= t.ctx;  // wave-uniform
+    const bool inside = SCORE != kScoreCap && t.tb >= t.left && t.tb + TS <= t.ctx;  // wave-uniform
     if (!inside) {
 #pragma unroll
       for (int h = 0; h < S::TG; ++h)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           float s = sc[h][r];
-          if constexpr (SOFTCAP) s = soft_cap(s * a.score_scale, a.softcap_log2);
+          if constexpr (SCORE == kScoreCap) s = soft_cap(s * a.score_scale, a.softcap_log2);
           const int key = t.tb + 16 * h + 4 * q + r;
           sc[h][r] = (key >= t.left && key < t.ctx) ? s : -INFINITY;
         }
@@ -789,8 +798,8 @@ __device__ __forceinline__ void decode_stream_body(StreamArgs sa) {
       for (int i = 0; i < 4 * S::TG; ++i) v[i] = sc[i >> 2][i & 3];
       mx = col4_max(tree_max(v));
     }
-    if (__builtin_amdgcn_ballot_w64(mx > (SOFTCAP ? m_run + kDecodeRescaleSlack : m_thr))) {
-      const float m_new = fmaxf(m_run, SOFTCAP ? mx : mx * a.score_scale);
+    if (__builtin_amdgcn_ballot_w64(mx > (LOG2 ? m_run + kDecodeRescaleSlack : m_thr))) {
+      const float m_new = fmaxf(m_run, LOG2 ? mx : mx * a.score_scale);
       const float alpha = m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_new);
       l_run *= alpha;
       m_run = m_new;
@@ -807,7 +816,7 @@ __device__ __forceinline__ void decode_stream_body(StreamArgs sa) {
     for (int h = 0; h < S::TG; ++h)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float p = SOFTCAP ? fast_exp2(sc[h][r] - m_base) : fast_exp2(__builtin_fmaf(sc[h][r], a.score_scale, -m_base));
+        const float p = LOG2 ? fast_exp2(sc[h][r] - m_base) : fast_exp2(__builtin_fmaf(sc[h][r], a.score_scale, -m_base));
         sc[h][r] = p;
         l_run += p;
       }
@@ -913,13 +922,13 @@ __device__ __forceinline__ void decode_stream_body(StreamArgs sa) {
   if (kMaxPend > 0 && npend == 2) flush(pend1);
 }
 
-template <int D, bool SOFTCAP, int MODE>
+template <int D, int SCORE, int MODE>
 __global__ __launch_bounds__(64, 1) void decode_stream_kernel(StreamArgs sa) {
-  decode_stream_body<D, SOFTCAP, MODE, kArithMfma>(sa);
+  decode_stream_body<D, SCORE, MODE, kArithMfma>(sa);
 }
-template <int D, bool SOFTCAP, int MODE>
+template <int D, int SCORE, int MODE>
 __global__ __launch_bounds__(64, 1) void decode_stream_dot_kernel(StreamArgs sa) {
-  decode_stream_body<D, SOFTCAP, MODE, kArithDot>(sa);
+  decode_stream_body<D, SCORE, MODE, kArithDot>(sa);
 }
 
 // ---------------------------------------------------------------------------
@@ -1023,10 +1032,10 @@ __global__ __launch_bounds__(64 * WAVES) void stream_merge_kernel(StreamMergeArg
   for (int e = 0; e < PER_LANE; ++e) dst[lane + 64 * e] = (uint16_t)bf16_bits(acc[e] * inv);
 }
 
-template <int D, bool SOFTCAP, int MODE>
+template <int D, int SCORE, int MODE>
 int resident_per_cu() {
   int n = 0;
-  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_stream_kernel<D, SOFTCAP, MODE>, 64, 0) !=
+  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_stream_kernel<D, SCORE, MODE>, 64, 0) !=
           hipSuccess ||
       n <= 0)
     n = 1;
@@ -1034,37 +1043,39 @@ int resident_per_cu() {
 }
 
 template <int D, int MODE>
-int resident_per_cu(bool softcap) {
-  return softcap ? resident_per_cu<D, true, MODE>() : resident_per_cu<D, false, MODE>();
+int resident_per_cu(int score) {
+  if (score == kScoreBias) return resident_per_cu<D, kScoreBias, MODE>();
+  return score == kScoreCap ? resident_per_cu<D, kScoreCap, MODE>() : resident_per_cu<D, kScorePlain, MODE>();
 }
 
 template <int D>
-int resident_per_cu(bool softcap, int mode) {
-  if (mode == kKeyBlocks) return resident_per_cu<D, kKeyBlocks>(softcap);
-  if (mode == kLoadBlocks) return resident_per_cu<D, kLoadBlocks>(softcap);
-  return resident_per_cu<D, kTileBlocks>(softcap);
+int resident_per_cu(int score, int mode) {
+  if (mode == kKeyBlocks) return resident_per_cu<D, kKeyBlocks>(score);
+  if (mode == kLoadBlocks) return resident_per_cu<D, kLoadBlocks>(score);
+  return resident_per_cu<D, kTileBlocks>(score);
 }
 
 template <int D, int MODE>
-void launch_stream_mode(const StreamArgs& sa, bool softcap, dim3 grid, hipStream_t stream) {
+void launch_stream_mode(const StreamArgs& sa, int score, dim3 grid, hipStream_t stream) {
 #if GK_STREAM_DOT
   if constexpr (D <= 128) {
-    if (sa.d.heads_per_group <= kDotMaxHeads) {
-      if (softcap) decode_stream_dot_kernel<D, true, MODE><<<grid, 64, 0, stream>>>(sa);
-      else decode_stream_dot_kernel<D, false, MODE><<<grid, 64, 0, stream>>>(sa);
+    if (sa.d.heads_per_group <= kDotMaxHeads && score != kScoreBias) {
+      if (score == kScoreCap) decode_stream_dot_kernel<D, kScoreCap, MODE><<<grid, 64, 0, stream>>>(sa);
+      else decode_stream_dot_kernel<D, kScorePlain, MODE><<<grid, 64, 0, stream>>>(sa);
       return;
     }
   }
 #endif
-  if (softcap) decode_stream_kernel<D, true, MODE><<<grid, 64, 0, stream>>>(sa);
-  else decode_stream_kernel<D, false, MODE><<<grid, 64, 0, stream>>>(sa);
+  if (score == kScoreBias) decode_stream_kernel<D, kScoreBias, MODE><<<grid, 64, 0, stream>>>(sa);
+  else if (score == kScoreCap) decode_stream_kernel<D, kScoreCap, MODE><<<grid, 64, 0, stream>>>(sa);
+  else decode_stream_kernel<D, kScorePlain, MODE><<<grid, 64, 0, stream>>>(sa);
 }
 
 template <int D>
-void launch_stream_kernel(const StreamArgs& sa, bool softcap, int mode, dim3 grid, hipStream_t stream) {
-  if (mode == kKeyBlocks) launch_stream_mode<D, kKeyBlocks>(sa, softcap, grid, stream);
-  else if (mode == kLoadBlocks) launch_stream_mode<D, kLoadBlocks>(sa, softcap, grid, stream);
-  else launch_stream_mode<D, kTileBlocks>(sa, softcap, grid, stream);
+void launch_stream_kernel(const StreamArgs& sa, int score, int mode, dim3 grid, hipStream_t stream) {
+  if (mode == kKeyBlocks) launch_stream_mode<D, kKeyBlocks>(sa, score, grid, stream);
+  else if (mode == kLoadBlocks) launch_stream_mode<D, kLoadBlocks>(sa, score, grid, stream);
+  else launch_stream_mode<D, kTileBlocks>(sa, score, grid, stream);
 }
 
 // Slot lookup of a block size (the kernel's MODE).
@@ -1079,21 +1090,21 @@ int device_cus();
 
 // Workgroups of the balanced grid: the CUs times the workgroups one CU keeps
 // resident (LDS-bound), queried once per device and kernel variant.
-int stream_decode_wgs(int head_dim, bool softcap, int block_size) {
+int stream_decode_wgs(int head_dim, int score, int block_size) {
   static std::mutex mu;
-  static int cached[64][3][2][3] = {};
+  static int cached[64][3][3][3] = {};
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) dev = 0;
   const int di = head_dim == 64 ? 0 : (head_dim == 128 ? 1 : 2);
   const int mode = block_mode(head_dim, block_size);
   std::lock_guard<std::mutex> lock(mu);
-  int& slot = cached[dev][di][softcap ? 1 : 0][mode];
+  int& slot = cached[dev][di][score][mode];
   if (!slot) {
     int per_cu = 1;
     switch (head_dim) {
-      case 64: per_cu = resident_per_cu<64>(softcap, mode); break;
-      case 128: per_cu = resident_per_cu<128>(softcap, mode); break;
-      default: per_cu = resident_per_cu<256>(softcap, mode); break;
+      case 64: per_cu = resident_per_cu<64>(score, mode); break;
+      case 128: per_cu = resident_per_cu<128>(score, mode); break;
+      default: per_cu = resident_per_cu<256>(score, mode); break;
     }
     slot = device_cus() * per_cu;
   }
@@ -1107,7 +1118,7 @@ size_t stream_decode_workspace_bytes(int head_dim, int heads_per_group, int64_t 
   return o_bytes + ml_bytes + (size_t)units * 2 * sizeof(float);
 }
 
-int launch_stream_decode(const DecodeArgs& a, bool softcap, int head_dim, int wgs, void* workspace,
+int launch_stream_decode(const DecodeArgs& a, int score, int head_dim, int wgs, void* workspace,
                          hipStream_t stream) {
   StreamArgs sa{};
   sa.d = a;
@@ -1126,9 +1137,9 @@ int launch_stream_decode(const DecodeArgs& a, bool softcap, int head_dim, int wg
   const dim3 grid(wgs);
   const int mode = block_mode(head_dim, 1 << a.block_shift);
   switch (head_dim) {
-    case 64: launch_stream_kernel<64>(sa, softcap, mode, grid, stream); break;
-    case 128: launch_stream_kernel<128>(sa, softcap, mode, grid, stream); break;
-    default: launch_stream_kernel<256>(sa, softcap, mode, grid, stream); break;
+    case 64: launch_stream_kernel<64>(sa, score, mode, grid, stream); break;
+    case 128: launch_stream_kernel<128>(sa, score, mode, grid, stream); break;
+    default: launch_stream_kernel<256>(sa, score, mode, grid, stream); break;
   }
   if (int rc = hip_status(hipGetLastError(), "gk_paged_decode stream launch")) return rc;
 

@@ -51,9 +51,10 @@ struct UnitArgs {
 };
 
 // WAVES: 8, or fewer for short rows of many units (unit_waves).
-template <int D, bool SOFTCAP, int WAVES>
+template <int D, int SCORE, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 1) void decode_unit_kernel(UnitArgs ua) {
   using S = MfmaShape<D>;
+  constexpr bool LOG2 = SCORE != kScorePlain;  // scores in log2 units before the maxima, not raw products
   constexpr int TS = S::TS, LOADS = S::LOADS, CPR = S::CPR;
   static_assert(16 * D * 4 <= 2 * S::TILE, "a wave's partial output fits its stage");
   __shared__ __attribute__((aligned(16))) char stage[WAVES][2][S::TILE];
@@ -104,6 +105,8 @@ __global__ __launch_bounds__(WAVES * 64, 1) void decode_unit_kernel(UnitArgs ua)
       qb[c] = __builtin_bit_cast(bf16x8_t, v);
     }
   }
+  [[maybe_unused]] float slope = 0.f;  // distance slope of head c16
+  if constexpr (SCORE == kScoreBias) slope = column_slope(a.slopes, head0, hv, c16);
   // Lanes 0 .. 2 CPR - 1 (and again the lanes after them) hold the pieces of a
   // new row's key and value heads.
   const bool key_lane = (lane & (2 * CPR - 1)) < CPR;
@@ -227,15 +230,17 @@ __global__ __launch_bounds__(WAVES * 64, 1) void decode_unit_kernel(UnitArgs ua)
 #pragma unroll
       for (int c = 0; c < S::NC; ++c) sc[g] = mfma32(kr[g][c], qb[c], sc[g]);
     }
-    if constexpr (!SOFTCAP) mfma_results_ready(sc);
-    const bool inside = !SOFTCAP && tb >= rt.left && tb + TS <= rt.ctx;
+    if constexpr (!LOG2) mfma_results_ready(sc);
+    if constexpr (SCORE == kScoreBias)
+      bias_scores(sc, a.score_scale, a.softcap_log2, slope, (float)(tb + 4 * q - rt.ctx + 1));
+    const bool inside = SCORE != kScoreCap && tb >= rt.left && tb + TS <= rt.ctx;
     if (!inside) {
 #pragma unroll
       for (int g = 0; g < S::TG; ++g)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           float s = sc[g][r];
-          if constexpr (SOFTCAP) s = soft_cap(s * a.score_scale, a.softcap_log2);
+          if constexpr (SCORE == kScoreCap) s = soft_cap(s * a.score_scale, a.softcap_log2);
           const int key = tb + 16 * g + 4 * q + r;
           sc[g][r] = (key >= rt.left && key < rt.ctx) ? s : -INFINITY;
         }
@@ -247,8 +252,8 @@ __global__ __launch_bounds__(WAVES * 64, 1) void decode_unit_kernel(UnitArgs ua)
       for (int i = 0; i < 4 * S::TG; ++i) v[i] = sc[i >> 2][i & 3];
       mx = col4_max(tree_max(v));
     }
-    if (__builtin_amdgcn_ballot_w64(mx > (SOFTCAP ? m_run + kDecodeRescaleSlack : m_thr))) {
-      const float m_new = fmaxf(m_run, SOFTCAP ? mx : mx * a.score_scale);
+    if (__builtin_amdgcn_ballot_w64(mx > (LOG2 ? m_run + kDecodeRescaleSlack : m_thr))) {
+      const float m_new = fmaxf(m_run, LOG2 ? mx : mx * a.score_scale);
       const float alpha = m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_new);
       l_run *= alpha;
       m_run = m_new;
@@ -265,7 +270,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void decode_unit_kernel(UnitArgs ua)
     for (int g = 0; g < S::TG; ++g)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float p = SOFTCAP ? fast_exp2(sc[g][r] - m_base) : fast_exp2(__builtin_fmaf(sc[g][r], a.score_scale, -m_base));
+        const float p = LOG2 ? fast_exp2(sc[g][r] - m_base) : fast_exp2(__builtin_fmaf(sc[g][r], a.score_scale, -m_base));
         sc[g][r] = p;
         l_run += p;
       }
@@ -418,7 +423,7 @@ int unit_waves(const gk_decode_params* p, int64_t units) {
 
 bool unit_decode_fits(const gk_decode_params* p, int64_t units) { return unit_waves(p, units) != 0; }
 
-int launch_unit_decode(const DecodeArgs& a, bool softcap, int head_dim, const gk_decode_params* p, bool store,
+int launch_unit_decode(const DecodeArgs& a, int score, int head_dim, const gk_decode_params* p, bool store,
                        hipStream_t stream) {
   UnitArgs ua{};
   ua.d = a;
@@ -437,8 +442,9 @@ int launch_unit_decode(const DecodeArgs& a, bool softcap, int head_dim, const gk
   const int waves = unit_waves(p, units);
   const auto launch_waves = [&](auto d, auto w) {
     constexpr int D = decltype(d)::value, W = decltype(w)::value;
-    if (softcap) decode_unit_kernel<D, true, W><<<grid, W * 64, 0, stream>>>(ua);
-    else decode_unit_kernel<D, false, W><<<grid, W * 64, 0, stream>>>(ua);
+    if (score == kScoreBias) decode_unit_kernel<D, kScoreBias, W><<<grid, W * 64, 0, stream>>>(ua);
+    else if (score == kScoreCap) decode_unit_kernel<D, kScoreCap, W><<<grid, W * 64, 0, stream>>>(ua);
+    else decode_unit_kernel<D, kScorePlain, W><<<grid, W * 64, 0, stream>>>(ua);
   };
   const auto launch = [&](auto d) {
     if (waves == 2) launch_waves(d, std::integral_constant<int, 2>{});

@@ -39,6 +39,41 @@ __device__ __forceinline__ float soft_cap(float x, float cap) {
   return __builtin_fmaf(-2.f * cap, r, cap);
 }
 
+// What a score becomes on its way from q . k to the softmax (the SCORE argument
+// of the attention kernels):
+//  kScorePlain  scaled inside the exponent, the maxima on raw products;
+//  kScoreCap    cap * tanh(q . k * scale / cap), in log2 units;
+//  kScoreBias   the scaled (and, with a cap, capped) product plus
+//               slope_head * (key position - query position), in log2 units:
+//               one fused multiply-add more than plain for the distance, one for
+//               the scale that no longer rides in the exponent.
+constexpr int kScorePlain = 0, kScoreCap = 1, kScoreBias = 2;
+
+// Scores of one lane's column (keys base + 16 g + r of tile group g, register
+// r) with the column's distance bias: `slope` in log2 units, `distance` the base
+// key's position less the query's. The distances are small whole numbers, exact
+// in fp32, and the bias of the row's own key is 0, so a bias is rounded relative
+// to a weight of 2^bias: what rounding loses grows with |bias| and weighs less
+// than it grows.
+template <int G>
+__device__ __forceinline__ void bias_scores(f32x4_t (&sc)[G], float scale, float cap_log2, float slope,
+                                            float distance) {
+  float mul = scale;
+  if (cap_log2 > 0.f) {  // uniform
+    mul = 1.f;
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sc[g][r] = soft_cap(sc[g][r] * scale, cap_log2);
+  }
+  const float b0 = slope * distance;
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      sc[g][r] = __builtin_fmaf(sc[g][r], mul, __builtin_fmaf(slope, (float)(16 * g + r), b0));
+}
+
 // Pool slot of key t from block ids staged in LDS: s_bt[i] is the block id of
 // block b0 + i (block size 2^shift).
 __device__ __forceinline__ int slot_of(const int32_t* s_bt, int b0, int shift, int t) {
@@ -263,6 +298,22 @@ __device__ __forceinline__ void lds_dma16_once(uint32_t lds, __amdgpu_buffer_rsr
 // cannot prove itself once LDS direct loads (memory writes) are in the loop.
 __device__ __forceinline__ int32_t scalar_load(const int32_t* p, int64_t i) {
   return ((const __attribute__((address_space(4))) int32_t*)p)[i];
+}
+
+__device__ __forceinline__ float scalar_load(const float* p, int64_t i) {
+  return ((const __attribute__((address_space(4))) float*)p)[i];
+}
+
+// Distance slope of column c16 of a 16-head group (log2 units), 0 past its `heads`: scalar loads, so that a
+// pipeline that counts its vector loads is left alone.
+__device__ __forceinline__ float column_slope(const float* slopes, int head0, int heads, int c16) {
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const float v = scalar_load(slopes, head0 + (j < heads ? j : heads - 1));
+    s = c16 == j && j < heads ? v : s;
+  }
+  return s * kLog2e;
 }
 
 // LDS byte address of a __shared__ object (or a pointer into one).

@@ -102,7 +102,7 @@ __device__ __forceinline__ int stage_block_ids(const DecodeArgs& a, const int32_
 // each other: partitions are uniform in size, so the GPU stays evenly loaded
 // however skewed the context lengths are, and the log-sum-exp merge combines
 // a row's partitions afterwards.
-template <int D, bool SOFTCAP>
+template <int D, int SCORE>
 __global__ __launch_bounds__(64, mfma_waves_per_simd<D>()) void decode_mfma_kernel(DecodeArgs a) {
   using S = MfmaShape<D>;
   // Two stages of K and V tiles (separate objects, so the compiler can tell a
@@ -139,6 +139,9 @@ __global__ __launch_bounds__(64, mfma_waves_per_simd<D>()) void decode_mfma_kern
     if (c16 < hv) v = load16(a.query + (int64_t)qrow * a.q_stride + (int64_t)(head0 + c16) * D + (4 * c + q) * 8);
     qb[c] = __builtin_bit_cast(bf16x8_t, v);
   }
+
+  [[maybe_unused]] float slope = 0.f;  // distance slope of head c16
+  if constexpr (SCORE == kScoreBias) slope = column_slope(a.slopes, head0, hv, c16);
 
   f32x4_t o[S::NO];
 #pragma unroll
@@ -224,14 +227,16 @@ __global__ __launch_bounds__(64, mfma_waves_per_simd<D>()) void decode_mfma_kern
       for (int c = 0; c < S::NC; ++c) sc[h] = mfma32(kr[h][c], qb[c], sc[h]);
     }
 
+    if constexpr (SCORE == kScoreBias)
+      bias_scores(sc, a.score_scale, a.softcap_log2, slope, (float)(tb + 4 * q - ctx + 1));
     float mx = -INFINITY;
 #pragma unroll
     for (int h = 0; h < S::TG; ++h)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float s;
-        if constexpr (SOFTCAP) s = soft_cap(sc[h][r] * a.score_scale, a.softcap_log2);
-        else s = sc[h][r] * a.score_scale;
+        float s = sc[h][r];
+        if constexpr (SCORE == kScoreCap) s = soft_cap(s * a.score_scale, a.softcap_log2);
+        else if constexpr (SCORE == kScorePlain) s *= a.score_scale;
         s = (tb + 16 * h + 4 * q + r < pr.t_end) ? s : -INFINITY;
         sc[h][r] = s;
         mx = fmaxf(mx, s);
@@ -373,7 +378,7 @@ __global__ __launch_bounds__(64, mfma_waves_per_simd<D>()) void decode_mfma_kern
 // ---------------------------------------------------------------------------
 // dot2 kernel (small groups)
 // ---------------------------------------------------------------------------
-template <int D, int G, bool SOFTCAP>
+template <int D, int G, int SCORE>
 __global__ __launch_bounds__(kWaves * 64) void decode_dot_kernel(DecodeArgs a) {
   constexpr int LPT = D / 16;                      // lanes per token
   constexpr int TPW = 64 / LPT;                    // tokens per wave step
@@ -418,6 +423,12 @@ __global__ __launch_bounds__(kWaves * 64) void decode_dot_kernel(DecodeArgs a) {
     }
   }
 
+  [[maybe_unused]] float slope[G] = {};  // distance slopes, log2 units
+  if constexpr (SCORE == kScoreBias) {
+#pragma unroll
+    for (int gh = 0; gh < G; ++gh) slope[gh] = a.slopes[min(head0 + gh, a.q_heads - 1)] * kLog2e;
+  }
+
   float m[G], l[G], o[G][16];
 #pragma unroll
   for (int gh = 0; gh < G; ++gh) {
@@ -458,9 +469,12 @@ __global__ __launch_bounds__(kWaves * 64) void decode_dot_kernel(DecodeArgs a) {
           acc = dot2(qb[gh][e], word(kb[u], e), acc);
         }
         acc = group_sum<LPT>(acc);
-        float s;
-        if constexpr (SOFTCAP) s = soft_cap(acc * a.score_scale, a.softcap_log2);
-        else s = acc * a.score_scale;
+        float s = acc * a.score_scale;
+        if constexpr (SCORE == kScoreCap) s = soft_cap(s, a.softcap_log2);
+        if constexpr (SCORE == kScoreBias) {
+          if (a.softcap_log2 > 0.f) s = soft_cap(s, a.softcap_log2);
+          s = __builtin_fmaf(slope[gh], (float)(tb + u * TPW + grp - ctx + 1), s);
+        }
         p[u][gh] = valid[u] ? s : -INFINITY;
       }
     }
@@ -659,24 +673,31 @@ void launch_merge_dispatch(int head_dim, const MergeArgs& m, hipStream_t stream)
 // Host side
 // ---------------------------------------------------------------------------
 template <int D, int G>
-void launch_dot(const DecodeArgs& a, bool softcap, dim3 grid, size_t lds, hipStream_t stream) {
-  if (softcap) decode_dot_kernel<D, G, true><<<grid, kWaves * 64, lds, stream>>>(a);
-  else decode_dot_kernel<D, G, false><<<grid, kWaves * 64, lds, stream>>>(a);
+void launch_dot(const DecodeArgs& a, int score, dim3 grid, size_t lds, hipStream_t stream) {
+  if (score == kScoreBias) decode_dot_kernel<D, G, kScoreBias><<<grid, kWaves * 64, lds, stream>>>(a);
+  else if (score == kScoreCap) decode_dot_kernel<D, G, kScoreCap><<<grid, kWaves * 64, lds, stream>>>(a);
+  else decode_dot_kernel<D, G, kScorePlain><<<grid, kWaves * 64, lds, stream>>>(a);
 }
 
 template <int D>
-void launch_dot_g(int g, const DecodeArgs& a, bool softcap, dim3 grid, size_t lds, hipStream_t stream) {
+void launch_dot_g(int g, const DecodeArgs& a, int score, dim3 grid, size_t lds, hipStream_t stream) {
   switch (g) {
-    case 1: launch_dot<D, 1>(a, softcap, grid, lds, stream); break;
-    case 2: launch_dot<D, 2>(a, softcap, grid, lds, stream); break;
-    default: launch_dot<D, 3>(a, softcap, grid, lds, stream); break;
+    case 1: launch_dot<D, 1>(a, score, grid, lds, stream); break;
+    case 2: launch_dot<D, 2>(a, score, grid, lds, stream); break;
+    default: launch_dot<D, 3>(a, score, grid, lds, stream); break;
   }
 }
 
 template <int D>
-void launch_mfma(const DecodeArgs& a, bool softcap, dim3 grid, size_t lds, hipStream_t stream) {
-  if (softcap) decode_mfma_kernel<D, true><<<grid, 64, lds, stream>>>(a);
-  else decode_mfma_kernel<D, false><<<grid, 64, lds, stream>>>(a);
+void launch_mfma(const DecodeArgs& a, int score, dim3 grid, size_t lds, hipStream_t stream) {
+  if (score == kScoreBias) decode_mfma_kernel<D, kScoreBias><<<grid, 64, lds, stream>>>(a);
+  else if (score == kScoreCap) decode_mfma_kernel<D, kScoreCap><<<grid, 64, lds, stream>>>(a);
+  else decode_mfma_kernel<D, kScorePlain><<<grid, 64, lds, stream>>>(a);
+}
+
+// The score variant of a call: a distance bias (slopes) carries a cap with it.
+int score_kind(const gk_decode_params* p, const float* slopes) {
+  return slopes ? kScoreBias : p->softcap > 0.f ? kScoreCap : kScorePlain;
 }
 
 // Query heads one workgroup computes for a kv head: the whole group up to 16
@@ -742,14 +763,14 @@ int device_cus() {
 // every row's tiles (at most max_context / TS + 2 with a window's offset)
 // times the units, plus the grid's workgroups, stay below 2^31 (the kernel's
 // own test, stream_tiles_fit); larger batches take the partitioned kernel.
-bool use_stream(const gk_decode_params* p) {
+bool use_stream(const gk_decode_params* p, int score) {
   const int group = p->q_heads / p->kv_heads;
   if (p->partition_tokens != 0) return false;
   const int hpw = heads_per_workgroup(group);
   const int64_t units = (int64_t)p->rows * p->kv_heads * ((group + hpw - 1) / hpw);
   const int ts = p->head_dim == 256 ? 16 : 32;
   return stream_tiles_fit(units, p->max_context, ts,
-                          stream_decode_wgs(p->head_dim, p->softcap > 0.f, p->block_size));
+                          stream_decode_wgs(p->head_dim, score, p->block_size));
 }
 
 int64_t stream_units(const gk_decode_params* p) {
@@ -762,13 +783,13 @@ int64_t stream_units(const gk_decode_params* p) {
 // which needs no workspace and no merge.
 bool use_unit(const gk_decode_params* p) { return p->partition_tokens == 0 && unit_decode_fits(p, stream_units(p)); }
 
-int32_t decode_schedule(const gk_decode_params* p) {
-  return use_unit(p) ? GK_DECODE_UNIT : use_stream(p) ? GK_DECODE_BALANCED : GK_DECODE_PARTITIONED;
+int32_t decode_schedule(const gk_decode_params* p, int score) {
+  return use_unit(p) ? GK_DECODE_UNIT : use_stream(p, score) ? GK_DECODE_BALANCED : GK_DECODE_PARTITIONED;
 }
 
-int32_t decode_partition(const gk_decode_params* p) {
+int32_t decode_partition(const gk_decode_params* p, int score) {
   if (p->partition_tokens > 0) return p->partition_tokens;
-  if (use_stream(p)) return 0;
+  if (use_stream(p, score)) return 0;
   const int group = p->q_heads / p->kv_heads;
   const int hpw = heads_per_workgroup(group);
   const int64_t units = (int64_t)p->rows * p->kv_heads * ((group + hpw - 1) / hpw);
@@ -789,27 +810,29 @@ int32_t decode_partition(const gk_decode_params* p) {
   return part;
 }
 
-int32_t decode_max_parts(const gk_decode_params* p) {
-  const int32_t part = decode_partition(p);
+int32_t decode_max_parts(const gk_decode_params* p, int score) {
+  const int32_t part = decode_partition(p, score);
   if (part == 0) return 1;
   return std::max<int32_t>(1, (p->max_context + part - 1) / part);
 }
 
-size_t decode_workspace_bytes(const gk_decode_params* p) {
-  if (p->rows > 0 && use_stream(p))
+size_t decode_workspace_bytes(const gk_decode_params* p, int score) {
+  if (p->rows > 0 && use_stream(p, score))
     return stream_decode_workspace_bytes(p->head_dim, heads_per_workgroup(p->q_heads / p->kv_heads), stream_units(p),
-                                         stream_decode_wgs(p->head_dim, p->softcap > 0.f, p->block_size));
-  const int32_t parts = decode_max_parts(p);
+                                         stream_decode_wgs(p->head_dim, score, p->block_size));
+  const int32_t parts = decode_max_parts(p, score);
   if (parts <= 1 || p->rows == 0) return 0;
   const size_t n = (size_t)p->rows * p->q_heads * parts;
   const size_t o_bytes = (n * p->head_dim * sizeof(float) + 255) & ~size_t{255};
   return o_bytes + n * 2 * sizeof(float);
 }
 
-int paged_decode(const gk_decode_params* p, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+int paged_decode(const gk_decode_params* p, const float* slopes, void* workspace, size_t workspace_bytes,
+                 hipStream_t stream) {
   if (int rc = validate(p)) return rc;
   if (p->rows == 0) return GK_OK;
-  const int32_t schedule = decode_schedule(p);
+  const int score = score_kind(p, slopes);
+  const int32_t schedule = decode_schedule(p, score);
   const bool unit = schedule == GK_DECODE_UNIT;
   bool unit_store = false;
   if (p->new_key) {
@@ -825,10 +848,10 @@ int paged_decode(const gk_decode_params* p, void* workspace, size_t workspace_by
                                  p->head_dim, stream))
       return rc;
   }
-  const int32_t part = decode_partition(p);
-  const int32_t max_parts = decode_max_parts(p);
+  const int32_t part = decode_partition(p, score);
+  const int32_t max_parts = decode_max_parts(p, score);
   // The unit kernel uses none of it; what a caller has to bring does not depend on that choice.
-  const size_t need = decode_workspace_bytes(p);
+  const size_t need = decode_workspace_bytes(p, score);
   if (need > workspace_bytes || (need && !workspace))
     return fail(GK_ERR_WORKSPACE, "gk_paged_decode: workspace too small (" + std::to_string(need) + " bytes needed)");
   const int group = p->q_heads / p->kv_heads;
@@ -850,6 +873,7 @@ int paged_decode(const gk_decode_params* p, void* workspace, size_t workspace_by
   a.group = group;
   a.heads_per_group = hpw;
   a.head_groups = (group + hpw - 1) / hpw;
+  a.slopes = slopes;
   const bool softcap = p->softcap > 0.f;
   a.score_scale = softcap ? p->scale / p->softcap : p->scale * kLog2e;
   a.softcap_log2 = p->softcap * kLog2e;
@@ -858,9 +882,9 @@ int paged_decode(const gk_decode_params* p, void* workspace, size_t workspace_by
   a.max_parts = max_parts;
   a.out = static_cast<uint16_t*>(p->out);
   a.out_stride = p->out_row_stride;
-  if (unit) return launch_unit_decode(a, softcap, p->head_dim, p, unit_store, stream);
+  if (unit) return launch_unit_decode(a, score, p->head_dim, p, unit_store, stream);
   if (schedule == GK_DECODE_BALANCED)
-    return launch_stream_decode(a, softcap, p->head_dim, stream_decode_wgs(p->head_dim, softcap, p->block_size), workspace,
+    return launch_stream_decode(a, score, p->head_dim, stream_decode_wgs(p->head_dim, score, p->block_size), workspace,
                                 stream);
   if (need) {
     const size_t n = (size_t)p->rows * p->q_heads * max_parts;
@@ -873,15 +897,15 @@ int paged_decode(const gk_decode_params* p, void* workspace, size_t workspace_by
   const dim3 grid(max_parts, p->kv_heads * a.head_groups, p->rows);
   if (use_mfma(group)) {
     switch (p->head_dim) {
-      case 64: launch_mfma<64>(a, softcap, grid, bt_lds, stream); break;
-      case 128: launch_mfma<128>(a, softcap, grid, bt_lds, stream); break;
-      default: launch_mfma<256>(a, softcap, grid, bt_lds, stream); break;
+      case 64: launch_mfma<64>(a, score, grid, bt_lds, stream); break;
+      case 128: launch_mfma<128>(a, score, grid, bt_lds, stream); break;
+      default: launch_mfma<256>(a, score, grid, bt_lds, stream); break;
     }
   } else {
     switch (p->head_dim) {
-      case 64: launch_dot_g<64>(hpw, a, softcap, grid, bt_lds, stream); break;
-      case 128: launch_dot_g<128>(hpw, a, softcap, grid, bt_lds, stream); break;
-      default: launch_dot_g<256>(hpw, a, softcap, grid, bt_lds, stream); break;
+      case 64: launch_dot_g<64>(hpw, a, score, grid, bt_lds, stream); break;
+      case 128: launch_dot_g<128>(hpw, a, score, grid, bt_lds, stream); break;
+      default: launch_dot_g<256>(hpw, a, score, grid, bt_lds, stream); break;
     }
   }
   if (int rc = hip_status(hipGetLastError(), "gk_paged_decode partition launch")) return rc;
@@ -970,7 +994,7 @@ int scratch_on_device(hipStream_t stream, void** out) {
 int paged_decode_scratch(const gk_decode_params* p, hipStream_t stream) {
   if (int rc = validate(p)) return rc;
   if (p->rows == 0) return GK_OK;
-  const size_t need = decode_workspace_bytes(p);
+  const size_t need = decode_workspace_bytes(p, score_kind(p, nullptr));
   if (need > GK_DECODE_SCRATCH_BYTES)
     return fail(GK_ERR_WORKSPACE, "gk_paged_decode_scratch: these parameters need " + std::to_string(need) +
                                       " bytes of workspace, more than the " + std::to_string(GK_DECODE_SCRATCH_BYTES) +
@@ -978,30 +1002,47 @@ int paged_decode_scratch(const gk_decode_params* p, hipStream_t stream) {
   void* workspace = nullptr;
   if (need)
     if (int rc = scratch_on_device(stream, &workspace)) return rc;
-  return paged_decode(p, workspace, need, stream);
+  return paged_decode(p, nullptr, workspace, need, stream);
 }
 
 }  // namespace gk
 
 extern "C" size_t gk_paged_decode_workspace_bytes(const gk_decode_params* params) {
-  return params && params->struct_size == sizeof(gk_decode_params) ? gk::decode_workspace_bytes(params) : 0;
+  return params && params->struct_size == sizeof(gk_decode_params)
+             ? gk::decode_workspace_bytes(params, gk::score_kind(params, nullptr))
+             : 0;
+}
+
+extern "C" size_t gk_paged_decode_alibi_workspace_bytes(const gk_decode_params* params) {
+  return params && params->struct_size == sizeof(gk_decode_params) ? gk::decode_workspace_bytes(params, gk::kScoreBias)
+                                                                   : 0;
 }
 
 extern "C" int32_t gk_paged_decode_partition_tokens(const gk_decode_params* params) {
-  return params && params->struct_size == sizeof(gk_decode_params) ? gk::decode_partition(params) : 0;
+  return params && params->struct_size == sizeof(gk_decode_params)
+             ? gk::decode_partition(params, gk::score_kind(params, nullptr))
+             : 0;
 }
 
 extern "C" int32_t gk_paged_decode_schedule(const gk_decode_params* params) {
   const bool known = params && params->struct_size == sizeof(gk_decode_params) && params->rows > 0 &&
                      params->kv_heads > 0 && params->q_heads >= params->kv_heads &&
                      (params->head_dim == 64 || params->head_dim == 128 || params->head_dim == 256);
-  return known ? gk::decode_schedule(params) : GK_DECODE_PARTITIONED;
+  return known ? gk::decode_schedule(params, gk::score_kind(params, nullptr)) : GK_DECODE_PARTITIONED;
 }
 
 extern "C" int gk_paged_decode(const gk_decode_params* params, void* workspace, size_t workspace_bytes,
                                hipStream_t stream) {
   gk::clear_error();
-  return gk::paged_decode(params, workspace, workspace_bytes, stream);
+  return gk::paged_decode(params, nullptr, workspace, workspace_bytes, stream);
+}
+
+extern "C" int gk_paged_decode_alibi(const gk_decode_params* params, const float* slopes, void* workspace,
+                                     size_t workspace_bytes, hipStream_t stream) {
+  gk::clear_error();
+  if (params && params->rows != 0 && !slopes)
+    return gk::fail(GK_ERR_INVALID_ARGUMENT, "gk_paged_decode_alibi: null slopes");
+  return gk::paged_decode(params, slopes, workspace, workspace_bytes, stream);
 }
 
 extern "C" int gk_split_k_merge(const float* partial_out, const float* partial_ml, const int32_t* part_count,

@@ -1,0 +1,264 @@
+// Work plan of a shared-prefix attention launch: which keys every workgroup and
+// every one-wave worker takes, and where its partial results go. Plain host
+// C++, built once per attention plan from lengths that the plan's owner has on
+// the host; the CPU tests compile it with g++.
+//
+// Rows come in groups whose rows hold the same slots for the group's first
+// `prefix` tokens. The group's columns, (row, head) pairs of one kv head, attend
+// those keys together: in tiles of up to prefill_tile_qrows columns (eight waves
+// on one K/V tile in LDS) or, where they are few, as one wave's columns. Behind
+// the prefix every run of rows (consecutive positions of one request) attends
+// its own keys. Both kinds of work are cut along their keys; each piece leaves
+// an unnormalised partial, and a second launch joins a row's partials.
+#pragma once
+
+#include <algorithm>
+#include <cstdint>
+#include <vector>
+
+#include "prefill_schedule.hpp"
+
+namespace gk {
+
+// A worker is one wave: at most shared_columns columns (two 16-column tiles; one
+// at head_dim 256, where two spill 77 registers), tiles of shared_tile_keys keys.
+constexpr int shared_columns(int head_dim) { return head_dim > 128 ? 16 : 32; }
+constexpr int shared_tile_keys(int head_dim) { return head_dim > 128 ? 16 : 32; }
+constexpr int kSharedWaves = 8;  // workers of a workgroup
+
+struct SharedRun {
+  int32_t first_row, rows, pos, group;
+};
+
+// A tile of a workgroup: compact rows first .. first + rows - 1, keys
+// [key_lo, key_hi) in `steps` steps of prefill_step_keys from key0 on.
+struct SharedTile {
+  int32_t first, rows, key_lo, key_hi, key0, steps, col, batch_row;
+};
+constexpr int kSharedTileWords = 8;
+// A stretch of one worker's keys: `cols` columns of the compact rows from `first`
+// on, key tiles tile0 .. tile0 + tiles - 1.
+struct SharedSegment {
+  int32_t first, cols, tile0, tiles, key_lo, key_hi, col, batch_row;
+};
+constexpr int kSharedSegmentWords = 8;
+// Where a row's partials are: columns pre_col + p pre_stride (p < pre_parts) of
+// its prefix, own_col + p own_stride of its own keys, one column a head.
+struct SharedMerge {
+  int32_t pre_col, pre_parts, pre_stride, own_col, own_parts, own_stride, batch_row, pad;
+};
+constexpr int kSharedMergeWords = 8;
+
+struct SharedPlan {
+  std::vector<int32_t> row_map, row_position, worker_segs;
+  std::vector<SharedMerge> merges;   // one per compact row
+  std::vector<SharedTile> tiles;     // longest first
+  std::vector<SharedSegment> segs;
+  int64_t cols = 0;                  // partial columns of one kv head
+  int32_t worker_groups = 0;         // workgroups of workers
+};
+
+// What the split weighs, in microseconds.
+struct SharedCost {
+  double step;        // a tile's step with all its waves busy, a quarter of it whatever the columns
+  double tile_start;  // a workgroup's start and end
+  double key_tile;    // a worker's key tile where latency bounds it
+  double bytes;       // of a worker's key tile
+};
+inline SharedCost shared_cost(int head_dim) {
+  if (head_dim == 64) return {0.6, 5.0, 1.8, 32 * 64 * 4.0};
+  if (head_dim == 128) return {1.7, 6.0, 2.2, 32 * 128 * 4.0};
+  return {1.3, 6.0, 2.2, 16 * 256 * 4.0};
+}
+constexpr double kSharedBandwidth = 5.8e6;  // bytes a microsecond that workers reach together
+
+// Work of one kv head before it is cut.
+struct SharedWork {
+  int32_t first, rows, key_lo, key_hi;  // compact rows and their keys
+  bool own;                             // a run's own keys (else its group's prefix)
+  int32_t units;                        // steps of a tile, key tiles of a worker
+  int32_t start;                        // first key, aligned
+};
+
+inline SharedPlan shared_plan(const SharedRun* runs, int count, const int32_t* group_prefix, int group, int kv_heads,
+                              int head_dim, int window, int cus) {
+  SharedPlan plan;
+  const int tile_cols = prefill_tile_qrows(head_dim), tile_rows = tile_cols / group;
+  const int step_keys = prefill_step_keys(head_dim), key_tile = shared_tile_keys(head_dim);
+  const int columns = shared_columns(head_dim);
+  std::vector<SharedWork> wide, narrow;
+  const auto add = [&](int first, int rows, int lo, int hi, bool own) {
+    // Heads beyond a worker's columns go to a workgroup's tile; so do more than two workers' columns.
+    if (lo >= hi) return;
+    SharedWork w{first, rows, lo, hi, own, 0, 0};
+    const bool tile = group > columns || rows * group > (own ? 2 * columns : columns);
+    if (tile) {
+      w.start = lo / step_keys * step_keys;
+      w.units = (hi - w.start + step_keys - 1) / step_keys;
+      wide.push_back(w);
+      return;
+    }
+    const int most = columns / group;  // rows of a worker
+    w.start = lo / key_tile * key_tile;
+    for (int r = 0; r < rows; r += most) {
+      w.first = first + r;
+      w.rows = std::min(most, rows - r);
+      if (own) w.key_hi = hi - (rows - r - w.rows);  // the slice's last row's own key
+      w.units = (w.key_hi - w.start + key_tile - 1) / key_tile;
+      narrow.push_back(w);
+    }
+  };
+  // Rows in the order of their runs; a group's rows are side by side.
+  for (int i = 0; i < count;) {
+    const int g = runs[i].group, first = (int)plan.row_map.size(), prefix = group_prefix[g];
+    for (; i < count && runs[i].group == g; ++i) {
+      const SharedRun& run = runs[i];
+      const int at = (int)plan.row_map.size();
+      for (int r = 0; r < run.rows; ++r) {
+        plan.row_map.push_back(run.first_row + r);
+        plan.row_position.push_back(run.pos + r);
+        plan.merges.push_back({0, 0, 0, 0, 0, 0, run.first_row + r, 0});
+      }
+      for (int r = 0; r < run.rows; r += tile_rows) {
+        const int nr = std::min(tile_rows, run.rows - r), pos = run.pos + r;
+        add(at + r, nr, std::max(prefix, window > 0 ? pos - window + 1 : 0), pos + nr, true);
+      }
+    }
+    const int rows = (int)plan.row_map.size() - first;
+    for (int r = 0; r < rows; r += tile_rows) {
+      const int nr = std::min(tile_rows, rows - r);
+      int lo = 0;
+      if (window > 0) {
+        lo = INT32_MAX;
+        for (int k = 0; k < nr; ++k) lo = std::min(lo, std::max(0, plan.row_position[first + r + k] - window + 1));
+      }
+      add(first + r, nr, lo, prefix, false);
+    }
+  }
+
+  // How many of a kv head's CUs take workers: the number with which both kinds
+  // of work, side by side, end soonest.
+  const SharedCost cost = shared_cost(head_dim);
+  const int slots = std::max(1, cus / kv_heads);
+  int64_t key_tiles = 0;
+  double steps = 0;
+  int longest = 0;
+  for (const auto& w : narrow) key_tiles += w.units;
+  const auto step_cost = [&](const SharedWork& w) {
+    const int waves = (w.rows * group + tile_cols / 8 - 1) / (tile_cols / 8);
+    return cost.step * (0.25 + 0.75 * waves / 8);
+  };
+  for (const auto& w : wide) {
+    steps += w.units * step_cost(w);
+    longest = std::max(longest, w.units);
+  }
+  int best = narrow.empty() ? 0 : slots;
+  if (!narrow.empty() && !wide.empty()) {
+    double best_time = 1e30;
+    for (int a = 1; a < slots || a == 1; ++a) {
+      const double rate = std::min(kSharedBandwidth, a * kv_heads * kSharedWaves * cost.bytes / cost.key_tile);
+      const double busy = key_tiles * cost.bytes * kv_heads / rate;
+      const double beside = steps / std::max(1, slots - a) + cost.tile_start;
+      const double time = std::max(busy, beside);
+      if (time < best_time) {
+        best_time = time;
+        best = a;
+      }
+    }
+  }
+  // Two key tiles a worker at least: each segment costs a partial and a start.
+  int workers = (int)std::min<int64_t>(int64_t{best} * kSharedWaves, std::max<int64_t>(1, (key_tiles + 1) / 2));
+  if (narrow.empty()) workers = 0;
+  const int tile_slots = std::max(1, slots - (workers + kSharedWaves - 1) / kSharedWaves);
+
+  const auto place = [&](const SharedWork& w, int parts) {
+    // Columns of the work's parts, a multiple of 16 each.
+    const int stride = (w.rows * group + 15) / 16 * 16;
+    const int64_t col = plan.cols;
+    plan.cols += int64_t{stride} * parts;
+    for (int r = 0; r < w.rows; ++r) {
+      SharedMerge& m = plan.merges[w.first + r];
+      const int32_t at = (int32_t)(col + int64_t{r} * group);
+      if (w.own) m.own_col = at, m.own_parts = parts, m.own_stride = stride;
+      else m.pre_col = at, m.pre_parts = parts, m.pre_stride = stride;
+    }
+    return col;
+  };
+
+  // Tiles: equal pieces of at most `most` steps, the fewest with which one round
+  // of workgroups holds all pieces; whole where there are more tiles than slots.
+  if (!wide.empty()) {
+    int lo = 4, hi = std::max(4, longest);
+    const auto pieces = [&](int most) {
+      int64_t sum = 0;
+      for (const auto& w : wide) sum += (w.units + most - 1) / most;
+      return sum;
+    };
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (pieces(mid) <= tile_slots) hi = mid;
+      else lo = mid + 1;
+    }
+    for (const auto& w : wide) {
+      const int parts = (w.units + lo - 1) / lo;
+      const int64_t col = place(w, parts);
+      const int stride = (w.rows * group + 15) / 16 * 16;
+      for (int p = 0, done = 0; p < parts; ++p) {
+        const int end = (int)(int64_t{w.units} * (p + 1) / parts);
+        plan.tiles.push_back({w.first, w.rows, w.key_lo, w.key_hi, w.start + done * step_keys, end - done,
+                              (int32_t)(col + int64_t{p} * stride), plan.row_map[w.first]});
+        done = end;
+      }
+    }
+    std::stable_sort(plan.tiles.begin(), plan.tiles.end(), [](const SharedTile& a, const SharedTile& b) {
+      if (a.steps != b.steps) return a.steps > b.steps;
+      return a.key0 < b.key0;  // pieces of one key range together: they read the same K/V
+    });
+  }
+
+  // Workers: all key tiles end to end, each piece after one position that stands
+  // for its start and end, in equal shares: the smallest with which the workers
+  // suffice.
+  if (workers) {
+    std::vector<int32_t> piece_ends, pieces_of;  // key tiles where each piece ends; pieces of each work
+    int64_t share = std::max<int64_t>(3, (key_tiles + (int64_t)narrow.size() + workers - 1) / workers);
+    for (;; share += std::max<int64_t>(1, share / 64)) {
+      piece_ends.clear();
+      pieces_of.clear();
+      plan.worker_segs.assign(1, 0);
+      int64_t room = share;
+      for (const auto& w : narrow) {
+        int pieces = 0;
+        for (int done = 0; done < w.units; ++pieces) {
+          if (room < 2) {
+            plan.worker_segs.push_back((int32_t)piece_ends.size());
+            room = share;
+          }
+          int take = (int)std::min<int64_t>(w.units - done, room - 1);
+          if (w.units - done - take == 1) ++take;  // no piece of one tile
+          done += take;
+          room -= take + 1;
+          piece_ends.push_back(done);
+        }
+        pieces_of.push_back(pieces);
+      }
+      plan.worker_segs.push_back((int32_t)piece_ends.size());
+      if ((int)plan.worker_segs.size() - 1 <= workers) break;
+    }
+    size_t at = 0;
+    for (size_t i = 0; i < narrow.size(); ++i) {
+      const SharedWork& w = narrow[i];
+      const int64_t col = place(w, pieces_of[i]);
+      const int stride = (w.rows * group + 15) / 16 * 16;
+      for (int p = 0, done = 0; p < pieces_of[i]; ++p, ++at) {
+        plan.segs.push_back({w.first, w.rows * group, w.start / key_tile + done, piece_ends[at] - done, w.key_lo,
+                             w.key_hi, (int32_t)(col + int64_t{p} * stride), plan.row_map[w.first]});
+        done = piece_ends[at];
+      }
+    }
+    plan.worker_groups = ((int)plan.worker_segs.size() - 1 + kSharedWaves - 1) / kSharedWaves;
+  }
+  return plan;
+}
+
+}  // namespace gk

@@ -5,7 +5,10 @@
 //   torch.classes.gaudirt.PagedMetadata   slot mapping, block tables, lengths
 //   torch.ops.gaudirt.paged_attn          KV store + attention over the pool
 //   torch.ops.gaudirt._paged_attn_validated
+//   torch.ops.gaudirt.shared_prefix_attn  the same for groups that share a prefix
+//   torch.ops.gaudirt.paged_attn_alibi    the same with a distance bias
 //   torch.ops.gaudirt._advance_decode_lengths
+//   torch.ops.gaudirt.extend_block_tables tables, map and slots from device lengths
 //   gaudirt_amd._C._allocate_paged_kv     head-major pool on the block allocator
 //   gaudirt_amd._C._allocate_paged_slots / _release_paged_slots   page allocator
 //
@@ -28,6 +31,7 @@
 #include <cmath>
 #include <cstring>
 #include <limits>
+#include <map>
 #include <memory>
 #include <mutex>
 #include <numeric>
@@ -269,6 +273,18 @@ const PlanInfo& plan_data(const at::Tensor& tensor) {
               "GaudiRT attention: invalid or expired metadata plan");
   return *static_cast<const PlanInfo*>(dp.get_context());
 }
+
+// Work of a shared_prefix_attn call, kept by the metadata beside its attention
+// plan: the list of gk_shared_prefix_attention and, for runs of rows that fill a
+// prefill tile by themselves, that of gk_paged_prefill_listed.
+struct SharedPrefixPlan {
+  at::Tensor words;  // both lists
+  gk_shared_prefix_list shared{};
+  gk_prefill_list prefill{};
+  int64_t prefill_uncut_offset = 0;
+  int32_t prefill_uncut_items = 0;
+  at::Tensor row_request;
+};
 
 // ---------------------------------------------------------------------------
 // PagedMetadata (src/bridge/paged_metadata.hpp:17-109). Host constructor
@@ -797,24 +813,9 @@ class PagedMetadata : public torch::CustomClassHolder {
     info->row_map_offset = append(dec_map);
     if (!seq_rows.empty()) {
       gk_prefill_list list{};
-      list.struct_size = sizeof(list);
-      // Room for the list at the first try on 256 CUs: building one of 3000 items takes 0.7 ms.
-      int64_t tiles = 0;
-      for (const int32_t rows : seq_rows)
-        tiles += gk::prefill_row_tiles(rows, static_cast<int>(query_heads / kv_heads), static_cast<int>(head_dim));
       const auto build = [&](auto list_build) {
-        work.resize(gk::prefill_words_bound(tiles, static_cast<int>(kv_heads), 256));
-        for (;;) {
-          const int rc = list_build(seq_first.data(), seq_rows.data(), seq_prefix.data(),
-                                    static_cast<int32_t>(seq_rows.size()), static_cast<int32_t>(query_heads),
-                                    static_cast<int32_t>(kv_heads), static_cast<int32_t>(head_dim),
-                                    static_cast<int32_t>(window), work.data(), static_cast<int64_t>(work.size()), &list);
-          const int64_t need = int64_t{8} * list.item_count + int64_t{4} * list.merge_count;
-          const bool short_of = rc == GK_ERR_WORKSPACE && need > static_cast<int64_t>(work.size());
-          if (!short_of) check_gk(rc, "GaudiRT attention: prefill work list");
-          work.resize(need);
-          if (!short_of) break;
-        }
+        build_prefill_list(list_build, seq_first, seq_rows, seq_prefix, query_heads, kv_heads, head_dim, window, work,
+                           list);
       };
       build(gk_prefill_list_build);
       info->prefill_items = list.item_count;
@@ -866,10 +867,144 @@ class PagedMetadata : public torch::CustomClassHolder {
     return plan;
   }
 
+  // Work of shared_prefix_attn: consecutive groups of group_rows[g] batch rows
+  // whose requests hold the same slots for their first group_prefix[g] tokens.
+  const SharedPrefixPlan& shared_prefix_plan(const std::vector<int64_t>& group_rows,
+                                             const std::vector<int64_t>& group_prefix, int64_t query_heads,
+                                             int64_t kv_heads, int64_t head_dim, int64_t sliding_window) {
+    const int64_t window = sliding_window > 0 ? sliding_window : -1;
+    std::vector<int64_t> key{window, query_heads, kv_heads, head_dim};
+    key.insert(key.end(), group_rows.begin(), group_rows.end());
+    key.insert(key.end(), group_prefix.begin(), group_prefix.end());
+    const auto cached = shared_plans_.find(key);
+    if (cached != shared_plans_.end()) return cached->second;
+    check_groups(group_rows, group_prefix);
+    SharedPrefixPlan plan;
+    if (query_heads / kv_heads > 128) return shared_plans_.emplace(std::move(key), std::move(plan)).first->second;
+    const int group = static_cast<int>(query_heads / kv_heads);
+    const int64_t tile_rows = std::max<int64_t>(1, gk::prefill_tile_qrows(static_cast<int>(head_dim)) / group);
+    // Runs, cut where groups meet. A run that fills a tile of the prefill kernel
+    // reads its keys once for all of the tile's columns already: it gains nothing
+    // from its group.
+    std::vector<int32_t> first, rows, pos, of_group, prefix(group_prefix.begin(), group_prefix.end());
+    std::vector<int32_t> chunk_first, chunk_rows, chunk_pos;
+    int64_t g = 0, group_end = group_rows.empty() ? 0 : group_rows[0];
+    for (const auto& run : sequences_) {
+      for (int64_t r = run.row; r < run.row + run.length;) {
+        while (r >= group_end) group_end += group_rows[++g];
+        const int64_t end = std::min<int64_t>(run.row + run.length, group_end);
+        const bool chunk = end - r >= tile_rows;
+        (chunk ? chunk_first : first).push_back(static_cast<int32_t>(r));
+        (chunk ? chunk_rows : rows).push_back(static_cast<int32_t>(end - r));
+        (chunk ? chunk_pos : pos).push_back(static_cast<int32_t>(run.prefix + (r - run.row)));
+        if (!chunk) of_group.push_back(static_cast<int32_t>(g));
+        r = end;
+      }
+    }
+    plan.shared.struct_size = sizeof(plan.shared);
+    plan.prefill.struct_size = sizeof(plan.prefill);
+    std::vector<int32_t> words, work;
+    const auto append = [&](const std::vector<int32_t>& v) {
+      while (words.size() % 4) words.push_back(0);
+      const auto offset = static_cast<int64_t>(words.size());
+      words.insert(words.end(), v.begin(), v.end());
+      return offset;
+    };
+    if (!rows.empty()) {
+      work.resize(64 * rows.size() + 8192);
+      for (;;) {
+        const int rc = gk_shared_prefix_list_build(
+            first.data(), rows.data(), pos.data(), of_group.data(), static_cast<int32_t>(rows.size()), prefix.data(),
+            static_cast<int32_t>(prefix.size()), static_cast<int32_t>(query_heads), static_cast<int32_t>(kv_heads),
+            static_cast<int32_t>(head_dim), static_cast<int32_t>(window), work.data(),
+            static_cast<int64_t>(work.size()), &plan.shared);
+        const bool short_of = rc == GK_ERR_WORKSPACE && plan.shared.word_count > static_cast<int64_t>(work.size());
+        if (!short_of) check_gk(rc, "GaudiRT shared-prefix attention: work list");
+        work.resize(plan.shared.word_count);
+        if (!short_of) break;
+      }
+      append(work);
+    }
+    int64_t items_at = 0, merges_at = 0;
+    if (!chunk_rows.empty()) {
+      const auto build = [&](auto list_build, gk_prefill_list& list) {
+        build_prefill_list(list_build, chunk_first, chunk_rows, chunk_pos, query_heads, kv_heads, head_dim, window, work,
+                           list);
+      };
+      build(gk_prefill_list_build, plan.prefill);
+      items_at = append(work);
+      merges_at = items_at + int64_t{8} * plan.prefill.item_count;
+      if (plan.prefill.merge_count) {
+        gk_prefill_list uncut{};
+        build(gk_prefill_list_build_uncut, uncut);
+        plan.prefill_uncut_items = uncut.item_count;
+        plan.prefill_uncut_offset = append(work);
+      }
+    }
+    plan.words = upload_words(words, static_cast<int64_t>(words.size()));
+    plan.row_request = requests_;
+    const int32_t* device = plan.words.data_ptr<int32_t>();
+    plan.shared.words = device;
+    plan.prefill.items = device + items_at;
+    plan.prefill.merges = device + merges_at;
+    plan.shared.row_request = plan.prefill.row_request = requests_.data_ptr<int32_t>();
+    return shared_plans_.emplace(std::move(key), std::move(plan)).first->second;
+  }
+
  private:
   struct Sequence {
     int32_t row, length, prefix;
   };
+
+  void check_groups(const std::vector<int64_t>& group_rows, const std::vector<int64_t>& group_prefix) const {
+    TORCH_CHECK(!group_rows.empty() && group_rows.size() == group_prefix.size(),
+                "GaudiRT shared-prefix attention: one row count and one prefix a group are required");
+    int64_t row = 0;
+    for (size_t g = 0; g < group_rows.size(); ++g) {
+      TORCH_CHECK(group_rows[g] > 0 && group_rows[g] <= rows_ - row && group_prefix[g] >= 0 &&
+                      group_prefix[g] < context_,
+                  "GaudiRT shared-prefix attention: group rows or prefix out of range");
+      for (int64_t r = row; r < row + group_rows[g]; ++r)
+        TORCH_CHECK(positions_h_[r] >= group_prefix[g],
+                    "GaudiRT shared-prefix attention: a row lies inside its group's prefix");
+      // The host's own copy of the request map says whether the prefix is shared;
+      // a device map is the caller's word.
+      if (!mapping_h_.empty()) {
+        const int32_t* shared = mapping_h_.data() + static_cast<int64_t>(requests_h_[row]) * context_;
+        for (int64_t r = row + 1; r < row + group_rows[g]; ++r)
+          if (requests_h_[r] != requests_h_[r - 1])
+            TORCH_CHECK(std::memcmp(shared, mapping_h_.data() + static_cast<int64_t>(requests_h_[r]) * context_,
+                                    group_prefix[g] * sizeof(int32_t)) == 0,
+                        "GaudiRT shared-prefix attention: the rows of a group do not share its prefix");
+      }
+      row += group_rows[g];
+    }
+    TORCH_CHECK(row == rows_, "GaudiRT shared-prefix attention: the groups do not cover the rows");
+  }
+
+  // The work list of these chunks in `work`, its counts in `list`.
+  template <class Build>
+  static void build_prefill_list(Build list_build, const std::vector<int32_t>& first, const std::vector<int32_t>& rows,
+                                 const std::vector<int32_t>& prefix, int64_t query_heads, int64_t kv_heads,
+                                 int64_t head_dim, int64_t window, std::vector<int32_t>& work, gk_prefill_list& list) {
+    list.struct_size = sizeof(list);
+    // Room for the list at the first try on 256 CUs: building one of 3000 items takes 0.7 ms.
+    int64_t tiles = 0;
+    for (const int32_t n : rows)
+      tiles += gk::prefill_row_tiles(n, static_cast<int>(query_heads / kv_heads), static_cast<int>(head_dim));
+    work.resize(gk::prefill_words_bound(tiles, static_cast<int>(kv_heads), 256));
+    for (;;) {
+      const int rc = list_build(first.data(), rows.data(), prefix.data(), static_cast<int32_t>(rows.size()),
+                                static_cast<int32_t>(query_heads), static_cast<int32_t>(kv_heads),
+                                static_cast<int32_t>(head_dim), static_cast<int32_t>(window), work.data(),
+                                static_cast<int64_t>(work.size()), &list);
+      const int64_t need = int64_t{8} * list.item_count + int64_t{4} * list.merge_count;
+      const bool short_of = rc == GK_ERR_WORKSPACE && need > static_cast<int64_t>(work.size());
+      if (!short_of) check_gk(rc, "GaudiRT attention: prefill work list");
+      work.resize(need);
+      if (!short_of) break;
+    }
+  }
 
   // The request map on the device: the device constructors' own input, or
   // (host constructor) the host copy, uploaded on the current stream on first use.
@@ -891,6 +1026,7 @@ class PagedMetadata : public torch::CustomClassHolder {
       last_token_indices_,
       model_positions_;
   std::unordered_map<int64_t, at::Tensor> plans_;
+  std::map<std::vector<int64_t>, SharedPrefixPlan> shared_plans_;
 };
 
 // Output storage of pow2(rows) rows rounded to 256 bytes, shaped [rows, width]
@@ -925,11 +1061,10 @@ struct RotarySpec {
   bool neox;
 };
 
-at::Tensor paged_attn_impl(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value,
-                           const at::Tensor& key_pool, const at::Tensor& value_pool, const at::Tensor& locations,
-                           const at::Tensor& plan_tensor, int64_t head_dim, double scale, double softcap,
-                           int64_t sliding_window, const RotarySpec* rotary) {
-  const auto& plan = plan_data(plan_tensor);
+// The entry checks of an attention call, all before any KV write.
+void check_attention(const PlanInfo& plan, const at::Tensor& query, const at::Tensor& key, const at::Tensor& value,
+                     const at::Tensor& key_pool, const at::Tensor& value_pool, const at::Tensor& locations,
+                     int64_t head_dim, double scale, double softcap, int64_t sliding_window) {
   const hipStream_t stream = current_stream();
   const float scale_f = static_cast<float>(scale), softcap_f = static_cast<float>(softcap);
   TORCH_CHECK(plan.stream == stream && std::isfinite(scale) && std::isfinite(scale_f) && scale_f > 0 &&
@@ -964,6 +1099,68 @@ at::Tensor paged_attn_impl(const at::Tensor& query, const at::Tensor& key, const
                   pool_address % 256 == 0 &&
                   pool_address - storage_base + 2 * value_offset <= pool_storage.nbytes(),
               "GaudiRT attention: KV pool descriptor is not backed by combined storage");
+}
+
+// What the prefill kernel's launches of one call have in common.
+gk_prefill_params prefill_params(const PlanInfo& plan, const at::Tensor& q, void* pool, const at::Tensor& output,
+                                 float scale, float softcap, int64_t sliding_window) {
+  const int32_t* words = plan.storage.data_ptr<int32_t>();
+  gk_prefill_params f{};
+  f.struct_size = sizeof(f);
+  f.query = q.data_ptr();
+  f.q_row_stride = q.stride(0);
+  f.pool = pool;
+  f.slots = plan.slots;
+  f.block_tables = plan.block_tables(words);
+  f.bt_stride = plan.bt_stride;
+  f.block_size = static_cast<int32_t>(plan.block_size);
+  f.q_heads = static_cast<int32_t>(plan.query_heads);
+  f.kv_heads = static_cast<int32_t>(plan.kv_heads);
+  f.head_dim = static_cast<int32_t>(plan.head_dim);
+  f.scale = scale;
+  f.softcap = softcap;
+  f.sliding_window = sliding_window > 0 ? static_cast<int32_t>(sliding_window) : -1;
+  f.out = output.data_ptr();
+  f.out_row_stride = output.stride(0);
+  return f;
+}
+
+// A prefill work list, cut or (without memory for the partials, or asked for) uncut.
+void launch_prefill_list(const gk_prefill_params& f, gk_prefill_list list, const int32_t* uncut_items,
+                         int32_t uncut_count, bool uncut, const at::Tensor& query, const float* slopes,
+                         hipStream_t stream) {
+  const auto take_uncut = [&] {
+    list.items = uncut_items;
+    list.item_count = uncut_count;
+    list.merge_count = list.part_slots = 0;
+  };
+  if (uncut && list.merge_count) take_uncut();
+  size_t need = gk_prefill_list_workspace_bytes(&f, &list);
+  at::Tensor workspace;
+  if (need) {
+    // Partials are worth some MiB of scratch, but no call fails for them.
+    try {
+      workspace = at::empty({static_cast<int64_t>(need)}, query.options().dtype(at::kByte));
+    } catch (const c10::OutOfMemoryError&) {
+      take_uncut();
+      need = 0;
+    }
+  }
+  void* const scratch = need ? workspace.data_ptr() : nullptr;
+  check_gk(slopes ? gk_paged_prefill_alibi(&f, &list, slopes, scratch, need, stream)
+                  : gk_paged_prefill_listed(&f, &list, scratch, need, stream),
+           "GaudiRT attention (prefill)");
+}
+
+at::Tensor paged_attn_impl(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value,
+                           const at::Tensor& key_pool, const at::Tensor& value_pool, const at::Tensor& locations,
+                           const at::Tensor& plan_tensor, int64_t head_dim, double scale, double softcap,
+                           int64_t sliding_window, const RotarySpec* rotary,
+                           const float* slopes = nullptr) {
+  const auto& plan = plan_data(plan_tensor);
+  const hipStream_t stream = current_stream();
+  const float scale_f = static_cast<float>(scale), softcap_f = static_cast<float>(softcap);
+  check_attention(plan, query, key, value, key_pool, value_pool, locations, head_dim, scale, softcap, sliding_window);
   record_pool_stream(key_pool, stream);
 
   auto q = kernel_rows(query);
@@ -1016,23 +1213,6 @@ at::Tensor paged_attn_impl(const at::Tensor& query, const at::Tensor& key, const
   const int32_t sw = sliding_window > 0 ? static_cast<int32_t>(sliding_window) : -1;
   const int32_t partition = g_decode_partition.load(std::memory_order_relaxed);  // > 0: batch-invariant
   if (plan.prefill_items) {
-    gk_prefill_params f{};
-    f.struct_size = sizeof(f);
-    f.query = q.data_ptr();
-    f.q_row_stride = q.stride(0);
-    f.pool = pool;
-    f.slots = plan.slots;
-    f.block_tables = plan.block_tables(words);
-    f.bt_stride = plan.bt_stride;
-    f.block_size = static_cast<int32_t>(plan.block_size);
-    f.q_heads = static_cast<int32_t>(plan.query_heads);
-    f.kv_heads = static_cast<int32_t>(plan.kv_heads);
-    f.head_dim = static_cast<int32_t>(head_dim);
-    f.scale = scale_f;
-    f.softcap = softcap_f;
-    f.sliding_window = sw;
-    f.out = output.data_ptr();
-    f.out_row_stride = output.stride(0);
     gk_prefill_list list{};
     list.struct_size = sizeof(list);
     list.items = words + plan.prefill_items_offset;
@@ -1041,25 +1221,9 @@ at::Tensor paged_attn_impl(const at::Tensor& query, const at::Tensor& key, const
     list.item_count = static_cast<int32_t>(plan.prefill_items);
     list.merge_count = static_cast<int32_t>(plan.prefill_merges);
     list.part_slots = static_cast<int32_t>(plan.prefill_part_slots);
-    const auto take_uncut = [&] {
-      list.items = words + plan.prefill_uncut_offset;
-      list.item_count = static_cast<int32_t>(plan.prefill_uncut_items);
-      list.merge_count = list.part_slots = 0;
-    };
-    if (partition > 0 && plan.prefill_merges) take_uncut();
-    size_t need = gk_prefill_list_workspace_bytes(&f, &list);
-    at::Tensor workspace;
-    if (need) {
-      // Partials are worth some MiB of scratch, but no call fails for them.
-      try {
-        workspace = at::empty({static_cast<int64_t>(need)}, query.options().dtype(at::kByte));
-      } catch (const c10::OutOfMemoryError&) {
-        take_uncut();
-        need = 0;
-      }
-    }
-    check_gk(gk_paged_prefill_listed(&f, &list, need ? workspace.data_ptr() : nullptr, need, stream),
-             "GaudiRT attention (prefill)");
+    launch_prefill_list(prefill_params(plan, q, pool, output, scale_f, softcap_f, sliding_window), list,
+                        words + plan.prefill_uncut_offset, static_cast<int32_t>(plan.prefill_uncut_items),
+                        partition > 0, query, slopes, stream);
   }
   if (plan.decode_rows) {
     gk_decode_params p{};
@@ -1091,10 +1255,12 @@ at::Tensor paged_attn_impl(const at::Tensor& query, const at::Tensor& key, const
       p.new_kv_row_stride = k.stride(0);
       p.slot_mapping = locations.data_ptr<int32_t>();
     }
-    const size_t need = gk_paged_decode_workspace_bytes(&p);
+    const size_t need = slopes ? gk_paged_decode_alibi_workspace_bytes(&p) : gk_paged_decode_workspace_bytes(&p);
     at::Tensor workspace;
     if (need) workspace = at::empty({static_cast<int64_t>(need)}, query.options().dtype(at::kByte));
-    check_gk(gk_paged_decode(&p, need ? workspace.data_ptr() : nullptr, need, stream), "GaudiRT attention");
+    void* const scratch = need ? workspace.data_ptr() : nullptr;
+    check_gk(slopes ? gk_paged_decode_alibi(&p, slopes, scratch, need, stream) : gk_paged_decode(&p, scratch, need, stream),
+             "GaudiRT attention");
   }
   return output;
 }
@@ -1127,6 +1293,72 @@ at::Tensor paged_attn(const at::Tensor& query, const at::Tensor& key, const at::
   return paged_attn_validated(query, key, value, key_pool, value_pool, metadata->row_locations(),
                               metadata->row_requests(), metadata->rotary_positions(), plan, metadata->rotary_header(),
                               head_dim, scale, softcap, sliding_window);
+}
+
+// The attention plan of a call with metadata (paged_attn's own steps).
+at::Tensor plan_for(const c10::intrusive_ptr<PagedMetadata>& metadata, const at::Tensor& query,
+                    const at::Tensor& key_pool, int64_t head_dim, int64_t sliding_window) {
+  TORCH_CHECK(metadata, "GaudiRT paged attention: metadata is required");
+  TORCH_CHECK(query.dim() == 2 && key_pool.dim() == 3 && (head_dim == 64 || head_dim == 128 || head_dim == 256),
+              "GaudiRT paged attention: invalid tensor ranks or head dimension");
+  const auto q_heads = query.size(1) / head_dim;
+  const auto kv_heads = key_pool.size(1);
+  return sliding_window > 0 ? metadata->attention_plan_for(q_heads, kv_heads, head_dim, sliding_window)
+                            : metadata->attention_plan(q_heads, kv_heads, head_dim);
+}
+
+// paged_attn with slopes[head] * (key position - query position) added to every
+// score after the scale and the softcap. No counterpart in the reference.
+at::Tensor paged_attn_alibi(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value,
+                            const at::Tensor& key_pool, const at::Tensor& value_pool,
+                            const c10::intrusive_ptr<PagedMetadata>& metadata, const at::Tensor& slopes,
+                            int64_t head_dim, double scale, double softcap, int64_t sliding_window) {
+  const auto plan = plan_for(metadata, query, key_pool, head_dim, sliding_window);
+  TORCH_CHECK(slopes.is_cuda() && slopes.device().index() == current_device() && slopes.scalar_type() == at::kFloat &&
+                  slopes.dim() == 1 && slopes.size(0) == query.size(1) / head_dim,
+              "GaudiRT attention: slopes must be one fp32 device value a query head");
+  const auto dense = slopes.contiguous();
+  return paged_attn_impl(query, key, value, key_pool, value_pool, metadata->row_locations(), plan, head_dim, scale,
+                         softcap, sliding_window, nullptr, dense.data_ptr<float>());
+}
+
+// paged_attn of groups of batch rows whose requests share a prefix: its keys are
+// read once for all rows of a group. No counterpart in the reference.
+at::Tensor shared_prefix_attn(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value,
+                              const at::Tensor& key_pool, const at::Tensor& value_pool,
+                              const c10::intrusive_ptr<PagedMetadata>& metadata, std::vector<int64_t> group_rows,
+                              std::vector<int64_t> group_prefix, int64_t head_dim, double scale, double softcap,
+                              int64_t sliding_window) {
+  const auto plan_tensor = plan_for(metadata, query, key_pool, head_dim, sliding_window);
+  const auto& plan = plan_data(plan_tensor);
+  const auto locations = metadata->row_locations();
+  check_attention(plan, query, key, value, key_pool, value_pool, locations, head_dim, scale, softcap, sliding_window);
+  const auto& work = metadata->shared_prefix_plan(group_rows, group_prefix, plan.query_heads, plan.kv_heads, head_dim,
+                                                  sliding_window);
+  // Batch-invariant calls attend every row by itself, and so do groups of more
+  // than 128 query heads a kv head, which fill the decode kernels alone.
+  if (g_decode_partition.load(std::memory_order_relaxed) > 0 || !work.shared.rows)
+    return paged_attn_impl(query, key, value, key_pool, value_pool, locations, plan_tensor, head_dim, scale, softcap,
+                           sliding_window, nullptr);
+  const hipStream_t stream = current_stream();
+  record_pool_stream(key_pool, stream);
+  const auto q = kernel_rows(query), k = kernel_rows(key), v = kernel_rows(value);
+  auto output = bucket_output(query, plan.rows, query.size(1));
+  void* pool = key_pool.data_ptr();
+  check_gk(gk_kv_store(k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), locations.data_ptr<int32_t>(),
+                       static_cast<int32_t>(plan.rows), pool, plan.slots, static_cast<int32_t>(plan.kv_heads),
+                       static_cast<int32_t>(head_dim), stream),
+           "GaudiRT attention: KV store");
+  const auto params = prefill_params(plan, q, pool, output, static_cast<float>(scale), static_cast<float>(softcap),
+                                     sliding_window);
+  const size_t need = gk_shared_prefix_workspace_bytes(&params, &work.shared);
+  const auto workspace = at::empty({static_cast<int64_t>(need)}, query.options().dtype(at::kByte));
+  check_gk(gk_shared_prefix_attention(&params, &work.shared, workspace.data_ptr(), need, stream),
+           "GaudiRT shared-prefix attention");
+  if (work.prefill.item_count)
+    launch_prefill_list(params, work.prefill, work.words.data_ptr<int32_t>() + work.prefill_uncut_offset,
+                        work.prefill_uncut_items, false, query, nullptr, stream);
+  return output;
 }
 
 // ---------------------------------------------------------------------------
@@ -1292,6 +1524,78 @@ std::tuple<at::Tensor, at::Tensor> advance_decode_lengths(const at::Tensor& seq_
   return {next, orig_next};
 }
 
+// extend_block_tables: a scheduler step's block tables, request map, slots and
+// positions from device lengths, with no host read. No counterpart in the
+// reference, whose scheduler fills its map on the host.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> extend_block_tables(
+    const at::Tensor& block_tables, const c10::optional<at::Tensor>& mapping, const at::Tensor& requests,
+    const at::Tensor& prefixes, const at::Tensor& lengths, const at::Tensor& free_pages,
+    const c10::optional<at::Tensor>& free_head, const c10::optional<at::Tensor>& parents, int64_t page_size,
+    int64_t slots, int64_t max_rows) {
+  const int device = current_device();
+  const auto table = [&](const at::Tensor& t) {
+    return t.is_cuda() && t.device().index() == device && t.scalar_type() == at::kInt && t.dim() == 2 &&
+           t.is_contiguous() && t.size(0) > 0 && t.size(1) > 0 && t.numel() <= std::numeric_limits<int32_t>::max();
+  };
+  const auto vector = [&](const at::Tensor& t) {
+    return t.is_cuda() && t.device().index() == device && t.dim() == 1 &&
+           (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong);
+  };
+  TORCH_CHECK(table(block_tables) && (!mapping || (table(*mapping) && mapping->size(0) == block_tables.size(0))),
+              "GaudiRT block tables: expected contiguous device int32 tables and a map of as many rows");
+  TORCH_CHECK(vector(requests) && vector(prefixes) && vector(lengths) && vector(free_pages) &&
+                  (!parents || vector(*parents)),
+              "GaudiRT block tables: expected device int32 or int64 vectors");
+  const int64_t batch = requests.numel();
+  TORCH_CHECK(batch <= GK_EXTEND_MAX_BATCH && prefixes.numel() == batch && lengths.numel() == batch &&
+                  prefixes.scalar_type() == lengths.scalar_type() &&
+                  (!parents || (parents->numel() == batch && parents->scalar_type() == requests.scalar_type())),
+              "GaudiRT block tables: sequence vectors do not match (at most ", GK_EXTEND_MAX_BATCH, " sequences)");
+  TORCH_CHECK(!free_head || (free_head->is_cuda() && free_head->device().index() == device &&
+                             free_head->scalar_type() == at::kInt && free_head->numel() == 1),
+              "GaudiRT block tables: the free list's head must be one device int32");
+  TORCH_CHECK(page_size >= 1 && page_size <= (1 << 20) && (page_size & (page_size - 1)) == 0 && slots > 0 &&
+                  slots <= std::numeric_limits<int32_t>::max() && max_rows >= 0 && max_rows <= (1 << 30) &&
+                  free_pages.numel() <= std::numeric_limits<int32_t>::max(),
+              "GaudiRT block tables: unsupported page size, slots, free pages or rows");
+  // Strided inputs are packed first (the kernel reads dense vectors).
+  const auto req = requests.contiguous(), pre = prefixes.contiguous(), len = lengths.contiguous(),
+             pages = free_pages.contiguous();
+  const auto par = parents ? parents->contiguous() : at::Tensor();
+  const auto words = block_tables.options();
+  auto locations = at::empty({max_rows}, words), row_requests = at::empty({max_rows}, words),
+       positions = at::empty({max_rows}, words), seq_lens = at::empty({batch}, len.options()),
+       counts = at::empty({4}, words);
+  gk_extend_params p{};
+  p.struct_size = sizeof(p);
+  p.block_tables = block_tables.data_ptr<int32_t>();
+  p.mapping = mapping ? mapping->data_ptr<int32_t>() : nullptr;
+  p.requests = static_cast<int32_t>(block_tables.size(0));
+  p.pages = static_cast<int32_t>(block_tables.size(1));
+  p.context = mapping ? static_cast<int32_t>(mapping->size(1)) : 0;
+  p.seq_requests = req.data_ptr();
+  p.prefixes = pre.data_ptr();
+  p.lengths = len.data_ptr();
+  p.parents = parents ? par.data_ptr() : nullptr;
+  p.free_pages = pages.data_ptr();
+  p.free_head = free_head ? free_head->data_ptr<int32_t>() : nullptr;
+  p.requests_int64 = req.scalar_type() == at::kLong;
+  p.lengths_int64 = len.scalar_type() == at::kLong;
+  p.pages_int64 = pages.scalar_type() == at::kLong;
+  p.free_count = pages.numel();
+  p.batch = static_cast<int32_t>(batch);
+  p.page_size = static_cast<int32_t>(page_size);
+  p.slots = slots;
+  p.max_rows = static_cast<int32_t>(max_rows);
+  p.out_locations = locations.data_ptr<int32_t>();
+  p.out_requests = row_requests.data_ptr<int32_t>();
+  p.out_positions = positions.data_ptr<int32_t>();
+  p.out_lengths = seq_lens.data_ptr();
+  p.counts = counts.data_ptr<int32_t>();
+  check_gk(gk_extend_block_tables(&p, current_stream()), "GaudiRT block tables");
+  return {locations, row_requests, positions, seq_lens, counts};
+}
+
 // ---------------------------------------------------------------------------
 // Paged slot allocator (src/bridge/paged_slot_allocator.cpp:91-190).
 // ---------------------------------------------------------------------------
@@ -1407,6 +1711,15 @@ TORCH_LIBRARY(gaudirt, m) {
   m.def("rotary_paged_attn(Tensor query, Tensor key, Tensor value, Tensor(a!) key_pool, Tensor(b!) value_pool, "
         "Tensor cache, __torch__.torch.classes.gaudirt.PagedMetadata metadata, int head_dim, int rotary_dim, "
         "bool is_neox, float scale, float softcap=0.0, int sliding_window=-1) -> Tensor");
+  m.def("shared_prefix_attn(Tensor query, Tensor key, Tensor value, Tensor(a!) key_pool, Tensor(b!) value_pool, "
+        "__torch__.torch.classes.gaudirt.PagedMetadata metadata, int[] group_rows, int[] group_prefix, int head_dim, "
+        "float scale, float softcap=0.0, int sliding_window=-1) -> Tensor");
+  m.def("paged_attn_alibi(Tensor query, Tensor key, Tensor value, Tensor(a!) key_pool, Tensor(b!) value_pool, "
+        "__torch__.torch.classes.gaudirt.PagedMetadata metadata, Tensor slopes, int head_dim, float scale, "
+        "float softcap=0.0, int sliding_window=-1) -> Tensor");
+  m.def("extend_block_tables(Tensor(a!) block_tables, Tensor(b!)? mapping, Tensor requests, Tensor prefixes, "
+        "Tensor lengths, Tensor free_pages, Tensor? free_head, Tensor? parents, int page_size, int slots, "
+        "int max_rows) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(gaudirt, CUDA, m) {
@@ -1417,6 +1730,9 @@ TORCH_LIBRARY_IMPL(gaudirt, CUDA, m) {
   m.impl("rotary_embedding_positions", TORCH_FN(gaudirt_amd::rotary_embedding_positions));
   m.impl("_rotary_embedding_validated", TORCH_FN(gaudirt_amd::rotary_embedding_validated));
   m.impl("rotary_paged_attn", TORCH_FN(gaudirt_amd::rotary_paged_attn));
+  m.impl("shared_prefix_attn", TORCH_FN(gaudirt_amd::shared_prefix_attn));
+  m.impl("paged_attn_alibi", TORCH_FN(gaudirt_amd::paged_attn_alibi));
+  m.impl("extend_block_tables", TORCH_FN(gaudirt_amd::extend_block_tables));
 }
 
 namespace gaudirt_amd {

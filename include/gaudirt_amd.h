@@ -223,6 +223,61 @@ int gk_paged_prefill_listed(const gk_prefill_params* params, const gk_prefill_li
                             size_t workspace_bytes, hipStream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Attention with a bias that falls with distance: gk_paged_decode and
+ * gk_paged_prefill_listed (same parameters, schedules and workspaces) with
+ *   score + slopes[head] * (key position - query position)
+ * after the scale and the optional softcap; slopes: fp32 [q_heads] on the
+ * device, finite. A row's own key has no bias; with a positive slope farther
+ * keys weigh less. No counterpart in the reference.
+ * ------------------------------------------------------------------------- */
+size_t gk_paged_decode_alibi_workspace_bytes(const gk_decode_params* params);
+int gk_paged_decode_alibi(const gk_decode_params* params, const float* slopes, void* workspace,
+                          size_t workspace_bytes, hipStream_t stream);
+int gk_paged_prefill_alibi(const gk_prefill_params* params, const gk_prefill_list* list, const float* slopes,
+                           void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Attention of rows whose requests share a prefix. Rows come in runs
+ * (run_rows[i] batch rows from run_first_row[i] on, at positions run_pos[i],
+ * run_pos[i] + 1, ... of one request), runs in groups (run_group, in ascending
+ * order). The requests of a group hold the same slots for their first
+ * group_prefix[g] tokens, and every row of the group lies behind them
+ * (run_pos >= group_prefix). Row results are gk_paged_prefill's, to rounding:
+ * the prefix's keys are read once for all rows of the group (through the block
+ * table of its first row's request) instead of once a row, and every key range
+ * leaves fp32 partials in the workspace, which a second launch merges
+ * (log-sum-exp). Where keys are cut depends on all rows of the list and on the
+ * GPU's CUs, and with it a row's last bits; the same list gives the same bits.
+ * No counterpart in the reference, which attends every row by itself.
+ *
+ * gk_shared_prefix_list_build (host only) plans the work of host-known lengths:
+ * it fills `list` but for its two pointers and writes word_count words
+ * (GK_ERR_WORKSPACE, with word_count set, when capacity is smaller). The caller
+ * copies the words to the device, 16-byte aligned, and sets words to the copy
+ * and row_request to the block-table row of every batch row (device).
+ * gk_shared_prefix_attention does not read seq_*, seqs and max_rows of its
+ * gk_prefill_params and writes the list's rows only; its sliding_window is the
+ * list's. Every key, the rows' own included, is in the pool (store first).
+ * A GQA group of at most 128; at most 65535 rows.
+ * ------------------------------------------------------------------------- */
+typedef struct gk_shared_prefix_list {
+  size_t struct_size;          /* sizeof(gk_shared_prefix_list) as the caller was built; checked */
+  const int32_t* words;
+  const int32_t* row_request;
+  int64_t part_cols;           /* partial results of one kv head */
+  int32_t rows, tile_count, workers, worker_groups, word_count;
+  int32_t map_at, position_at, merges_at, tiles_at, workers_at, segments_at;  /* sections of the words */
+} gk_shared_prefix_list;
+
+int gk_shared_prefix_list_build(const int32_t* run_first_row, const int32_t* run_rows, const int32_t* run_pos,
+                                const int32_t* run_group, int32_t runs, const int32_t* group_prefix, int32_t groups,
+                                int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t sliding_window,
+                                int32_t* words, int64_t capacity, gk_shared_prefix_list* list);
+size_t gk_shared_prefix_workspace_bytes(const gk_prefill_params* params, const gk_shared_prefix_list* list);
+int gk_shared_prefix_attention(const gk_prefill_params* params, const gk_shared_prefix_list* list, void* workspace,
+                               size_t workspace_bytes, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Split-K merge on its own: combines `parts` fp32 partial states per (row, head)
  * into bf16 output. partial_out [rows, heads, max_parts, head_dim] holds
  * unnormalised sums sum_t 2^(s_t - m) v_t; partial_ml [rows, heads, max_parts, 2]
@@ -384,6 +439,63 @@ int gk_metadata_normalize(const gk_metadata_params* params, void* workspace, siz
  * (src/bridge/attention_plan.cpp:36-57) for page-aligned maps. */
 int gk_block_tables(const int32_t* mapping, int32_t requests, int32_t context, int32_t page_size,
                     int32_t* tables, int32_t pages, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Block tables, token map and slots of a scheduler step from device lengths: no
+ * host read, no host list, safe to capture and replay (inputs are read at
+ * execution). No counterpart in the reference, whose scheduler fills its request
+ * map on the host.
+ *
+ * Sequence s (s < batch <= GK_EXTEND_MAX_BATCH) is row seq_requests[s] of the
+ * tables, holds prefixes[s] tokens and gets lengths[s] (>= 0) more. Its new
+ * pages come from free_pages[*free_head] on, in batch order. Written: the new
+ * entries of block_tables [requests, pages] and, when given, the new tokens'
+ * slots of mapping [requests, context]; per new token, in batch order, slot,
+ * request and position (max_rows each; rows behind the last token get slot -1,
+ * which gk_kv_store skips, request 0 and position 0); out_lengths[s] =
+ * prefixes[s] + lengths[s]; counts = {new tokens, *free_head + pages taken,
+ * status, sequence}. A sequence with parents[s] >= 0 (NULL or negative: none)
+ * starts from the first prefixes[s] tokens, whole pages, of that row: they are
+ * copied into its own row's table and map first. A page outside the pool
+ * ([0, slots / page_size)) is entered as -1, and its tokens get slot -1.
+ *
+ * The rows of a batch are distinct, and a parent holds the tokens before the
+ * call (it may itself get more in it). Status 0, or the first sequence in batch
+ * order that cannot be served, and why; nothing but rows of slot -1, unchanged
+ * out_lengths and counts {0, *free_head, ...} is then written:
+ *   1 its row, or its parent, outside [0, requests)
+ *   2 a negative length, or more tokens than a row of the tables (or map) holds
+ *   3 a parent and a prefix that is not whole pages, or its own row as parent
+ *   4 more new tokens than max_rows
+ *   5 the free list is exhausted
+ * ------------------------------------------------------------------------- */
+#define GK_EXTEND_MAX_BATCH 8192
+
+typedef struct gk_extend_params {
+  size_t struct_size;            /* sizeof(gk_extend_params) as the caller was built; checked */
+  int32_t* block_tables;         /* [requests, pages] */
+  int32_t* mapping;              /* [requests, context] or NULL */
+  int32_t requests, pages, context;
+  const void* seq_requests;      /* [batch] int32 or int64 (requests_int64) */
+  const void* prefixes;          /* [batch] int32 or int64 (lengths_int64) */
+  const void* lengths;           /* [batch] */
+  const void* parents;           /* [batch] as seq_requests, or NULL */
+  const void* free_pages;        /* [free_count] int32 or int64 (pages_int64) */
+  const int32_t* free_head;      /* [1], or NULL for 0 */
+  int32_t requests_int64, lengths_int64, pages_int64;
+  int64_t free_count;
+  int32_t batch;
+  int32_t page_size;             /* a power of two */
+  int64_t slots;
+  int32_t max_rows;
+  int32_t* out_locations;        /* [max_rows] */
+  int32_t* out_requests;         /* [max_rows] */
+  int32_t* out_positions;        /* [max_rows] */
+  void* out_lengths;             /* [batch] as lengths */
+  int32_t* counts;               /* [4] */
+} gk_extend_params;
+
+int gk_extend_block_tables(const gk_extend_params* params, hipStream_t stream);
 
 /* ---------------------------------------------------------------------------
  * Paged slot allocator (gk_paged_alloc_i32_v1 / gk_paged_free_i32_v1 of
