@@ -135,6 +135,12 @@ template <int D, int SCORE, int MODE, class Args>
 __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) {
   using S = PrefillShape<D>;
   constexpr bool SHARED = std::is_same_v<Args, SharedArgs>;
+  // Room between a base and the maximum that set it. A causal tile takes it above the base (a re-base when a score
+  // exceeds the base by it: probabilities of up to 2^8), a shared one below (the base lies that far above the
+  // maximum: up to 1), so that its unnormalised sums overflow only where the values' own sum does. Powers of two: the
+  // results are the same.
+  constexpr float kAbove = SHARED ? 0.f : kLazyRescale;
+  [[maybe_unused]] constexpr float kBelow = kLazyRescale;
   static_assert(!SHARED || SCORE != kScoreBias, "a shared tile's rows keep no distances");
   constexpr bool LOG2 = SCORE != kScorePlain;  // scores in log2 units before the maxima, not raw products
   // This head dimension's query tiles per wave (in place of the namespace's).
@@ -589,15 +595,17 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
     if constexpr (kNT % 2) mx[kNT - 1] = col4_max(mx[kNT - 1]);
     bool any = false;
 #pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) any = any || (mx[nt] > (LOG2 ? m_run[nt] + kLazyRescale : m_thr[nt]));
+    for (int nt = 0; nt < kNT; ++nt) any = any || (mx[nt] > (LOG2 ? m_run[nt] + kAbove : m_thr[nt]));
     if (__builtin_amdgcn_ballot_w64(any)) {
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
-        if (!__builtin_amdgcn_ballot_w64(mx[nt] > (LOG2 ? m_run[nt] + kLazyRescale : m_thr[nt]))) continue;
-        const float m_new = fmaxf(m_run[nt], LOG2 ? mx[nt] : mx[nt] * a.score_scale);
+        if (!__builtin_amdgcn_ballot_w64(mx[nt] > (LOG2 ? m_run[nt] + kAbove : m_thr[nt]))) continue;
+        float top = LOG2 ? mx[nt] : mx[nt] * a.score_scale;
+        if constexpr (SHARED) top += kBelow;
+        const float m_new = fmaxf(m_run[nt], top);
         const float alpha = m_run[nt] == -INFINITY ? 0.f : fast_exp2(m_run[nt] - m_new);
         m_run[nt] = m_new;
-        m_thr[nt] = (m_new + kLazyRescale) * inv_scale;
+        m_thr[nt] = (m_new + kAbove) * inv_scale;
         m_base[nt] = m_new == -INFINITY ? 0.f : m_new;
         if constexpr (!kMfmaSum) l_run[nt][0] *= alpha;
         // o rows are qrows 4q + r; qrow h's factor lives in lanes with c16 == h.

@@ -143,7 +143,7 @@ int shared_prefix_list_build(const int32_t* run_first_row, const int32_t* run_ro
   if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads ||
       q_heads / kv_heads > 128)
     return bad("invalid head geometry (GQA group at most 128)");
-  if (runs <= 0 || runs > 65535 || groups <= 0 || groups > runs || capacity < 0 || !run_first_row || !run_rows ||
+  if (runs <= 0 || runs > 65535 || groups <= 0 || groups > 65535 || capacity < 0 || !run_first_row || !run_rows ||
       !run_pos || !run_group || !group_prefix)
     return bad("invalid runs or groups");
   int64_t rows = 0;

@@ -964,6 +964,11 @@ class PagedMetadata : public torch::CustomClassHolder {
       TORCH_CHECK(group_rows[g] > 0 && group_rows[g] <= rows_ - row && group_prefix[g] >= 0 &&
                       group_prefix[g] < context_,
                   "GaudiRT shared-prefix attention: group rows or prefix out of range");
+      row += group_rows[g];
+    }
+    TORCH_CHECK(row == rows_, "GaudiRT shared-prefix attention: the groups do not cover the rows");
+    row = 0;
+    for (size_t g = 0; g < group_rows.size(); ++g) {
       for (int64_t r = row; r < row + group_rows[g]; ++r)
         TORCH_CHECK(positions_h_[r] >= group_prefix[g],
                     "GaudiRT shared-prefix attention: a row lies inside its group's prefix");
@@ -979,7 +984,6 @@ class PagedMetadata : public torch::CustomClassHolder {
       }
       row += group_rows[g];
     }
-    TORCH_CHECK(row == rows_, "GaudiRT shared-prefix attention: the groups do not cover the rows");
   }
 
   // The work list of these chunks in `work`, its counts in `list`.
