@@ -142,10 +142,10 @@ constexpr int kDotMaxHeads = 3;
 template <int D, int SCORE, int MODE, int ARITH>
 __device__ __forceinline__ void decode_stream_body(StreamArgs sa) {
   using S = MfmaShape<D>;
-  constexpr bool LOG2 = SCORE != kScorePlain;  // scores in log2 units before the maxima, not raw products
+  constexpr bool LOG2 = score_capped(SCORE);  // scores in log2 units before the maxima, not raw products
   constexpr int TS = S::TS;
   constexpr bool DOT = ARITH == kArithDot;
-  static_assert(!DOT || SCORE != kScoreBias, "the dot form has no distance bias");
+  static_assert(!DOT || !score_biased(SCORE), "the dot form has no distance bias");
   static_assert(!DOT || TS == 32, "the dot form pairs each key with two lanes (head_dim 64/128)");
   constexpr int DNC = D / 16;  // dot form: 16-byte chunks of a key row per lane (half the row)
   constexpr int DOD = D / 64;  // dot form: output dims per lane
@@ -740,9 +740,9 @@ __device__ __forceinline__ void decode_stream_body(StreamArgs sa) {
         l_run = 0.f;
         m_thr = -INFINITY;
         m_base = 0.f;
-        if constexpr (SCORE == kScoreBias) {
+        if constexpr (score_biased(SCORE)) {
           const int kvh = kv_head_of(t), hg = t.h - kvh * a.head_groups;
-          slope = column_slope(a.slopes, kvh * a.group + hg * 16, min(16, a.group - hg * 16), c16);
+          slope = column_slope(a.slopes, LOG2 ? 1.f : a.score_scale, kvh * a.group + hg * 16, min(16, a.group - hg * 16), c16);
         }
       }
     }
@@ -764,29 +764,29 @@ __device__ __forceinline__ void decode_stream_body(StreamArgs sa) {
         kr[h][c] = *reinterpret_cast<const bf16x8_t*>(kt + tt * (2 * D) + (((4 * c + q) ^ swz(tt, D / 8)) << 4));
     }
     f32x4_t sc[S::TG];
+    [[maybe_unused]] const float distance = (float)(t.tb + 4 * q - t.ctx + 1);
 #pragma unroll
     for (int h = 0; h < S::TG; ++h) {
-      sc[h] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      sc[h] = SCORE == kScoreBias ? bias4(slope, distance, h) : f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < S::NC; ++c) sc[h] = mfma32(kr[h][c], qb[c], sc[h]);
     }
 
     if constexpr (!LOG2) mfma_results_ready(sc);
-    if constexpr (SCORE == kScoreBias)
-      bias_scores(sc, a.score_scale, a.softcap_log2, slope, (float)(t.tb + 4 * q - t.ctx + 1));
 
     // Mask, and the row maximum over this lane's scores. Without softcap the
     // scores stay raw: a tile whose keys are all visible needs no per-element
     // mask, the maximum is compared with (m_run + kDecodeRescaleSlack) / scale
     // (kept with m_run), and the scale folds into the exponent below.
-    const bool inside = SCORE != kScoreCap && t.tb >= t.left && t.tb + TS <= t.ctx;  // wave-uniform
+    const bool inside = !LOG2 && t.tb >= t.left && t.tb + TS <= t.ctx;  // wave-uniform
     if (!inside) {
 #pragma unroll
       for (int h = 0; h < S::TG; ++h)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           float s = sc[h][r];
-          if constexpr (SCORE == kScoreCap) s = soft_cap(s * a.score_scale, a.softcap_log2);
+          if constexpr (LOG2) s = soft_cap(s * a.score_scale, a.softcap_log2);
+          if constexpr (SCORE == kScoreCapBias) s += bias4(slope, distance, h)[r];
           const int key = t.tb + 16 * h + 4 * q + r;
           sc[h][r] = (key >= t.left && key < t.ctx) ? s : -INFINITY;
         }
@@ -799,7 +799,9 @@ __device__ __forceinline__ void decode_stream_body(StreamArgs sa) {
       mx = col4_max(tree_max(v));
     }
     if (__builtin_amdgcn_ballot_w64(mx > (LOG2 ? m_run + kDecodeRescaleSlack : m_thr))) {
-      const float m_new = fmaxf(m_run, LOG2 ? mx : mx * a.score_scale);
+      float top = LOG2 ? mx : mx * a.score_scale;
+      if constexpr (SCORE == kScoreBias) top = base_above(top);
+      const float m_new = fmaxf(m_run, top);
       const float alpha = m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_new);
       l_run *= alpha;
       m_run = m_new;
@@ -1045,6 +1047,7 @@ int resident_per_cu() {
 template <int D, int MODE>
 int resident_per_cu(int score) {
   if (score == kScoreBias) return resident_per_cu<D, kScoreBias, MODE>();
+  if (score == kScoreCapBias) return resident_per_cu<D, kScoreCapBias, MODE>();
   return score == kScoreCap ? resident_per_cu<D, kScoreCap, MODE>() : resident_per_cu<D, kScorePlain, MODE>();
 }
 
@@ -1059,7 +1062,7 @@ template <int D, int MODE>
 void launch_stream_mode(const StreamArgs& sa, int score, dim3 grid, hipStream_t stream) {
 #if GK_STREAM_DOT
   if constexpr (D <= 128) {
-    if (sa.d.heads_per_group <= kDotMaxHeads && score != kScoreBias) {
+    if (sa.d.heads_per_group <= kDotMaxHeads && !score_biased(score)) {
       if (score == kScoreCap) decode_stream_dot_kernel<D, kScoreCap, MODE><<<grid, 64, 0, stream>>>(sa);
       else decode_stream_dot_kernel<D, kScorePlain, MODE><<<grid, 64, 0, stream>>>(sa);
       return;
@@ -1067,6 +1070,7 @@ void launch_stream_mode(const StreamArgs& sa, int score, dim3 grid, hipStream_t 
   }
 #endif
   if (score == kScoreBias) decode_stream_kernel<D, kScoreBias, MODE><<<grid, 64, 0, stream>>>(sa);
+  else if (score == kScoreCapBias) decode_stream_kernel<D, kScoreCapBias, MODE><<<grid, 64, 0, stream>>>(sa);
   else if (score == kScoreCap) decode_stream_kernel<D, kScoreCap, MODE><<<grid, 64, 0, stream>>>(sa);
   else decode_stream_kernel<D, kScorePlain, MODE><<<grid, 64, 0, stream>>>(sa);
 }
@@ -1092,7 +1096,7 @@ int device_cus();
 // resident (LDS-bound), queried once per device and kernel variant.
 int stream_decode_wgs(int head_dim, int score, int block_size) {
   static std::mutex mu;
-  static int cached[64][3][3][3] = {};
+  static int cached[64][3][4][3] = {};
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) dev = 0;
   const int di = head_dim == 64 ? 0 : (head_dim == 128 ? 1 : 2);

@@ -54,7 +54,7 @@ struct UnitArgs {
 template <int D, int SCORE, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 1) void decode_unit_kernel(UnitArgs ua) {
   using S = MfmaShape<D>;
-  constexpr bool LOG2 = SCORE != kScorePlain;  // scores in log2 units before the maxima, not raw products
+  constexpr bool LOG2 = score_capped(SCORE);  // scores in log2 units before the maxima, not raw products
   constexpr int TS = S::TS, LOADS = S::LOADS, CPR = S::CPR;
   static_assert(16 * D * 4 <= 2 * S::TILE, "a wave's partial output fits its stage");
   __shared__ __attribute__((aligned(16))) char stage[WAVES][2][S::TILE];
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void decode_unit_kernel(UnitArgs ua)
     }
   }
   [[maybe_unused]] float slope = 0.f;  // distance slope of head c16
-  if constexpr (SCORE == kScoreBias) slope = column_slope(a.slopes, head0, hv, c16);
+  if constexpr (score_biased(SCORE)) slope = column_slope(a.slopes, LOG2 ? 1.f : a.score_scale, head0, hv, c16);
   // Lanes 0 .. 2 CPR - 1 (and again the lanes after them) hold the pieces of a
   // new row's key and value heads.
   const bool key_lane = (lane & (2 * CPR - 1)) < CPR;
@@ -224,23 +224,23 @@ __global__ __launch_bounds__(WAVES * 64, 1) void decode_unit_kernel(UnitArgs ua)
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (more) issue(next, krs, kt);
     f32x4_t sc[S::TG];
+    [[maybe_unused]] const float distance = (float)(tb + 4 * q - rt.ctx + 1);
 #pragma unroll
     for (int g = 0; g < S::TG; ++g) {
-      sc[g] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      sc[g] = SCORE == kScoreBias ? bias4(slope, distance, g) : f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < S::NC; ++c) sc[g] = mfma32(kr[g][c], qb[c], sc[g]);
     }
     if constexpr (!LOG2) mfma_results_ready(sc);
-    if constexpr (SCORE == kScoreBias)
-      bias_scores(sc, a.score_scale, a.softcap_log2, slope, (float)(tb + 4 * q - rt.ctx + 1));
-    const bool inside = SCORE != kScoreCap && tb >= rt.left && tb + TS <= rt.ctx;
+    const bool inside = !LOG2 && tb >= rt.left && tb + TS <= rt.ctx;
     if (!inside) {
 #pragma unroll
       for (int g = 0; g < S::TG; ++g)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           float s = sc[g][r];
-          if constexpr (SCORE == kScoreCap) s = soft_cap(s * a.score_scale, a.softcap_log2);
+          if constexpr (LOG2) s = soft_cap(s * a.score_scale, a.softcap_log2);
+          if constexpr (SCORE == kScoreCapBias) s += bias4(slope, distance, g)[r];
           const int key = tb + 16 * g + 4 * q + r;
           sc[g][r] = (key >= rt.left && key < rt.ctx) ? s : -INFINITY;
         }
@@ -253,7 +253,9 @@ __global__ __launch_bounds__(WAVES * 64, 1) void decode_unit_kernel(UnitArgs ua)
       mx = col4_max(tree_max(v));
     }
     if (__builtin_amdgcn_ballot_w64(mx > (LOG2 ? m_run + kDecodeRescaleSlack : m_thr))) {
-      const float m_new = fmaxf(m_run, LOG2 ? mx : mx * a.score_scale);
+      float top = LOG2 ? mx : mx * a.score_scale;
+      if constexpr (SCORE == kScoreBias) top = base_above(top);
+      const float m_new = fmaxf(m_run, top);
       const float alpha = m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_new);
       l_run *= alpha;
       m_run = m_new;
@@ -443,6 +445,7 @@ int launch_unit_decode(const DecodeArgs& a, int score, int head_dim, const gk_de
   const auto launch_waves = [&](auto d, auto w) {
     constexpr int D = decltype(d)::value, W = decltype(w)::value;
     if (score == kScoreBias) decode_unit_kernel<D, kScoreBias, W><<<grid, W * 64, 0, stream>>>(ua);
+    else if (score == kScoreCapBias) decode_unit_kernel<D, kScoreCapBias, W><<<grid, W * 64, 0, stream>>>(ua);
     else if (score == kScoreCap) decode_unit_kernel<D, kScoreCap, W><<<grid, W * 64, 0, stream>>>(ua);
     else decode_unit_kernel<D, kScorePlain, W><<<grid, W * 64, 0, stream>>>(ua);
   };

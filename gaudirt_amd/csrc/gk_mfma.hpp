@@ -41,37 +41,37 @@ __device__ __forceinline__ float soft_cap(float x, float cap) {
 
 // What a score becomes on its way from q . k to the softmax (the SCORE argument
 // of the attention kernels):
-//  kScorePlain  scaled inside the exponent, the maxima on raw products;
-//  kScoreCap    cap * tanh(q . k * scale / cap), in log2 units;
-//  kScoreBias   the scaled (and, with a cap, capped) product plus
-//               slope_head * (key position - query position), in log2 units:
-//               one fused multiply-add more than plain for the distance, one for
-//               the scale that no longer rides in the exponent.
-constexpr int kScorePlain = 0, kScoreCap = 1, kScoreBias = 2;
+//  kScorePlain    scaled inside the exponent, the maxima on raw products;
+//  kScoreCap      cap * tanh(q . k * scale / cap), in log2 units;
+//  kScoreBias     plain plus slope_head * (key position - query position), in
+//                 the raw product's units so that the scale still rides in the
+//                 exponent: decode starts its accumulators from it, prefill adds
+//                 it where the maxima are taken;
+//  kScoreCapBias  kScoreCap plus slope_head * distance.
+constexpr int kScorePlain = 0, kScoreCap = 1, kScoreBias = 2, kScoreCapBias = 3;
+constexpr bool score_capped(int score) { return score == kScoreCap || score == kScoreCapBias; }
+constexpr bool score_biased(int score) { return score == kScoreBias || score == kScoreCapBias; }
 
-// Scores of one lane's column (keys base + 16 g + r of tile group g, register
-// r) with the column's distance bias: `slope` in log2 units, `distance` the base
-// key's position less the query's. The distances are small whole numbers, exact
-// in fp32, and the bias of the row's own key is 0, so a bias is rounded relative
-// to a weight of 2^bias: what rounding loses grows with |bias| and weighs less
-// than it grows.
-template <int G>
-__device__ __forceinline__ void bias_scores(f32x4_t (&sc)[G], float scale, float cap_log2, float slope,
-                                            float distance) {
-  float mul = scale;
-  if (cap_log2 > 0.f) {  // uniform
-    mul = 1.f;
+// The bias of the four keys of tile group g in one lane's column: `slope` in the
+// score's units, `distance` the lane's first key's position less the column's
+// query's. The distances are small whole numbers, exact in fp32, and the bias of the
+// row's own key is 0, so a bias is rounded relative to a weight of 2^bias: what
+// rounding loses grows with |bias| and weighs less than it grows.
+__device__ __forceinline__ f32x4_t bias4(float slope, float distance, int g) {
+  f32x4_t b;
 #pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) sc[g][r] = soft_cap(sc[g][r] * scale, cap_log2);
-  }
-  const float b0 = slope * distance;
-#pragma unroll
-  for (int g = 0; g < G; ++g)
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      sc[g][r] = __builtin_fmaf(sc[g][r], mul, __builtin_fmaf(slope, (float)(16 * g + r), b0));
+  for (int r = 0; r < 4; ++r) b[r] = slope * (distance + (float)(16 * g + r));
+  return b;
+}
+
+// A slope of 2^20 leaves a row its own key alone, and so does any larger one.
+constexpr float kMostSlope = 1048576.f;
+
+// A base for probabilities exp2(fma(score, scale, -base)) from the rounded product m of the largest score and the
+// scale: above it by more than the rounding of m, and of a part of the scores of size `part`, so that no probability
+// of a far piece (biases of 2^30 and more) passes 1 for the product's rounding. -inf stays.
+__device__ __forceinline__ float base_above(float m, float part = 0.f) {
+  return m == -INFINITY ? m : __builtin_fmaf(__builtin_fabsf(m) + __builtin_fabsf(part), 0x1p-22f, m);
 }
 
 // Pool slot of key t from block ids staged in LDS: s_bt[i] is the block id of
@@ -304,16 +304,16 @@ __device__ __forceinline__ float scalar_load(const float* p, int64_t i) {
   return ((const __attribute__((address_space(4))) float*)p)[i];
 }
 
-// Distance slope of column c16 of a 16-head group (log2 units), 0 past its `heads`: scalar loads, so that a
-// pipeline that counts its vector loads is left alone.
-__device__ __forceinline__ float column_slope(const float* slopes, int head0, int heads, int c16) {
+// Distance slope of column c16 of a 16-head group, in log2 units over `scale` (1 behind a cap, else what scales the
+// raw products), 0 past its `heads`: scalar loads, so that a pipeline that counts its vector loads is left alone.
+__device__ __forceinline__ float column_slope(const float* slopes, float scale, int head0, int heads, int c16) {
   float s = 0.f;
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     const float v = scalar_load(slopes, head0 + (j < heads ? j : heads - 1));
     s = c16 == j && j < heads ? v : s;
   }
-  return s * kLog2e;
+  return fminf(s, kMostSlope) * (kLog2e / scale);
 }
 
 // LDS byte address of a __shared__ object (or a pointer into one).

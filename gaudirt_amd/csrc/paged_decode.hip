@@ -141,7 +141,7 @@ __global__ __launch_bounds__(64, mfma_waves_per_simd<D>()) void decode_mfma_kern
   }
 
   [[maybe_unused]] float slope = 0.f;  // distance slope of head c16
-  if constexpr (SCORE == kScoreBias) slope = column_slope(a.slopes, head0, hv, c16);
+  if constexpr (score_biased(SCORE)) slope = column_slope(a.slopes, SCORE == kScoreBias ? a.score_scale : 1.f, head0, hv, c16);
 
   f32x4_t o[S::NO];
 #pragma unroll
@@ -220,23 +220,22 @@ __global__ __launch_bounds__(64, mfma_waves_per_simd<D>()) void decode_mfma_kern
 
     // S^T = K.Q^T: lane (q, c16) gets head c16, tokens tb + 16h + 4q + r.
     f32x4_t sc[S::TG];
+    [[maybe_unused]] const float distance = (float)(tb + 4 * q - ctx + 1);
 #pragma unroll
     for (int h = 0; h < S::TG; ++h) {
-      sc[h] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      sc[h] = SCORE == kScoreBias ? bias4(slope, distance, h) : f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < S::NC; ++c) sc[h] = mfma32(kr[h][c], qb[c], sc[h]);
     }
 
-    if constexpr (SCORE == kScoreBias)
-      bias_scores(sc, a.score_scale, a.softcap_log2, slope, (float)(tb + 4 * q - ctx + 1));
     float mx = -INFINITY;
 #pragma unroll
     for (int h = 0; h < S::TG; ++h)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float s = sc[h][r];
-        if constexpr (SCORE == kScoreCap) s = soft_cap(s * a.score_scale, a.softcap_log2);
-        else if constexpr (SCORE == kScorePlain) s *= a.score_scale;
+        float s = sc[h][r] * a.score_scale;
+        if constexpr (score_capped(SCORE)) s = soft_cap(s, a.softcap_log2);
+        if constexpr (SCORE == kScoreCapBias) s += bias4(slope, distance, h)[r];
         s = (tb + 16 * h + 4 * q + r < pr.t_end) ? s : -INFINITY;
         sc[h][r] = s;
         mx = fmaxf(mx, s);
@@ -424,9 +423,9 @@ __global__ __launch_bounds__(kWaves * 64) void decode_dot_kernel(DecodeArgs a) {
   }
 
   [[maybe_unused]] float slope[G] = {};  // distance slopes, log2 units
-  if constexpr (SCORE == kScoreBias) {
+  if constexpr (score_biased(SCORE)) {
 #pragma unroll
-    for (int gh = 0; gh < G; ++gh) slope[gh] = a.slopes[min(head0 + gh, a.q_heads - 1)] * kLog2e;
+    for (int gh = 0; gh < G; ++gh) slope[gh] = fminf(a.slopes[min(head0 + gh, a.q_heads - 1)], kMostSlope) * kLog2e;
   }
 
   float m[G], l[G], o[G][16];
@@ -470,11 +469,8 @@ __global__ __launch_bounds__(kWaves * 64) void decode_dot_kernel(DecodeArgs a) {
         }
         acc = group_sum<LPT>(acc);
         float s = acc * a.score_scale;
-        if constexpr (SCORE == kScoreCap) s = soft_cap(s, a.softcap_log2);
-        if constexpr (SCORE == kScoreBias) {
-          if (a.softcap_log2 > 0.f) s = soft_cap(s, a.softcap_log2);
-          s = __builtin_fmaf(slope[gh], (float)(tb + u * TPW + grp - ctx + 1), s);
-        }
+        if constexpr (score_capped(SCORE)) s = soft_cap(s, a.softcap_log2);
+        if constexpr (score_biased(SCORE)) s = __builtin_fmaf(slope[gh], (float)(tb + u * TPW + grp - ctx + 1), s);
         p[u][gh] = valid[u] ? s : -INFINITY;
       }
     }
@@ -675,6 +671,7 @@ void launch_merge_dispatch(int head_dim, const MergeArgs& m, hipStream_t stream)
 template <int D, int G>
 void launch_dot(const DecodeArgs& a, int score, dim3 grid, size_t lds, hipStream_t stream) {
   if (score == kScoreBias) decode_dot_kernel<D, G, kScoreBias><<<grid, kWaves * 64, lds, stream>>>(a);
+  else if (score == kScoreCapBias) decode_dot_kernel<D, G, kScoreCapBias><<<grid, kWaves * 64, lds, stream>>>(a);
   else if (score == kScoreCap) decode_dot_kernel<D, G, kScoreCap><<<grid, kWaves * 64, lds, stream>>>(a);
   else decode_dot_kernel<D, G, kScorePlain><<<grid, kWaves * 64, lds, stream>>>(a);
 }
@@ -691,13 +688,13 @@ void launch_dot_g(int g, const DecodeArgs& a, int score, dim3 grid, size_t lds, 
 template <int D>
 void launch_mfma(const DecodeArgs& a, int score, dim3 grid, size_t lds, hipStream_t stream) {
   if (score == kScoreBias) decode_mfma_kernel<D, kScoreBias><<<grid, 64, lds, stream>>>(a);
+  else if (score == kScoreCapBias) decode_mfma_kernel<D, kScoreCapBias><<<grid, 64, lds, stream>>>(a);
   else if (score == kScoreCap) decode_mfma_kernel<D, kScoreCap><<<grid, 64, lds, stream>>>(a);
   else decode_mfma_kernel<D, kScorePlain><<<grid, 64, lds, stream>>>(a);
 }
 
-// The score variant of a call: a distance bias (slopes) carries a cap with it.
-int score_kind(const gk_decode_params* p, const float* slopes) {
-  return slopes ? kScoreBias : p->softcap > 0.f ? kScoreCap : kScorePlain;
+int score_kind(const gk_decode_params* p, bool biased) {
+  return p->softcap > 0.f ? (biased ? kScoreCapBias : kScoreCap) : biased ? kScoreBias : kScorePlain;
 }
 
 // Query heads one workgroup computes for a kv head: the whole group up to 16
@@ -831,7 +828,7 @@ int paged_decode(const gk_decode_params* p, const float* slopes, void* workspace
                  hipStream_t stream) {
   if (int rc = validate(p)) return rc;
   if (p->rows == 0) return GK_OK;
-  const int score = score_kind(p, slopes);
+  const int score = score_kind(p, slopes != nullptr);
   const int32_t schedule = decode_schedule(p, score);
   const bool unit = schedule == GK_DECODE_UNIT;
   bool unit_store = false;
@@ -994,7 +991,7 @@ int scratch_on_device(hipStream_t stream, void** out) {
 int paged_decode_scratch(const gk_decode_params* p, hipStream_t stream) {
   if (int rc = validate(p)) return rc;
   if (p->rows == 0) return GK_OK;
-  const size_t need = decode_workspace_bytes(p, score_kind(p, nullptr));
+  const size_t need = decode_workspace_bytes(p, score_kind(p, false));
   if (need > GK_DECODE_SCRATCH_BYTES)
     return fail(GK_ERR_WORKSPACE, "gk_paged_decode_scratch: these parameters need " + std::to_string(need) +
                                       " bytes of workspace, more than the " + std::to_string(GK_DECODE_SCRATCH_BYTES) +
@@ -1009,18 +1006,19 @@ int paged_decode_scratch(const gk_decode_params* p, hipStream_t stream) {
 
 extern "C" size_t gk_paged_decode_workspace_bytes(const gk_decode_params* params) {
   return params && params->struct_size == sizeof(gk_decode_params)
-             ? gk::decode_workspace_bytes(params, gk::score_kind(params, nullptr))
+             ? gk::decode_workspace_bytes(params, gk::score_kind(params, false))
              : 0;
 }
 
 extern "C" size_t gk_paged_decode_alibi_workspace_bytes(const gk_decode_params* params) {
-  return params && params->struct_size == sizeof(gk_decode_params) ? gk::decode_workspace_bytes(params, gk::kScoreBias)
-                                                                   : 0;
+  return params && params->struct_size == sizeof(gk_decode_params)
+             ? gk::decode_workspace_bytes(params, gk::score_kind(params, true))
+             : 0;
 }
 
 extern "C" int32_t gk_paged_decode_partition_tokens(const gk_decode_params* params) {
   return params && params->struct_size == sizeof(gk_decode_params)
-             ? gk::decode_partition(params, gk::score_kind(params, nullptr))
+             ? gk::decode_partition(params, gk::score_kind(params, false))
              : 0;
 }
 
@@ -1028,7 +1026,7 @@ extern "C" int32_t gk_paged_decode_schedule(const gk_decode_params* params) {
   const bool known = params && params->struct_size == sizeof(gk_decode_params) && params->rows > 0 &&
                      params->kv_heads > 0 && params->q_heads >= params->kv_heads &&
                      (params->head_dim == 64 || params->head_dim == 128 || params->head_dim == 256);
-  return known ? gk::decode_schedule(params, gk::score_kind(params, nullptr)) : GK_DECODE_PARTITIONED;
+  return known ? gk::decode_schedule(params, gk::score_kind(params, false)) : GK_DECODE_PARTITIONED;
 }
 
 extern "C" int gk_paged_decode(const gk_decode_params* params, void* workspace, size_t workspace_bytes,

@@ -127,6 +127,7 @@ __global__ __launch_bounds__(64) void prefill_merge_kernel(PrefillMergeArgs a) {
 template <int D, int MODE>
 void launch_mode(const PrefillArgs& a, int score, dim3 grid, hipStream_t stream) {
   if (score == kScoreBias) prefill_kernel<D, kScoreBias, MODE, PrefillArgs><<<grid, kPrefillWaves * 64, 0, stream>>>(a);
+  else if (score == kScoreCapBias) prefill_kernel<D, kScoreCapBias, MODE, PrefillArgs><<<grid, kPrefillWaves * 64, 0, stream>>>(a);
   else if (score == kScoreCap) prefill_kernel<D, kScoreCap, MODE, PrefillArgs><<<grid, kPrefillWaves * 64, 0, stream>>>(a);
   else prefill_kernel<D, kScorePlain, MODE, PrefillArgs><<<grid, kPrefillWaves * 64, 0, stream>>>(a);
 }
@@ -145,7 +146,7 @@ namespace {
 
 int launch_prefill(const gk_prefill_params* p, const PrefillArgs& a, int64_t workgroups, hipStream_t stream) {
   const dim3 grid((unsigned)workgroups);
-  const int score = a.slopes ? kScoreBias : p->softcap > 0.f ? kScoreCap : kScorePlain;
+  const int score = p->softcap > 0.f ? (a.slopes ? kScoreCapBias : kScoreCap) : a.slopes ? kScoreBias : kScorePlain;
   if (p->head_dim == 64) launch<64>(a, score, p->block_size, grid, stream);
   else if (p->head_dim == 128) launch<128>(a, score, p->block_size, grid, stream);
   else launch<256>(a, score, p->block_size, grid, stream);

@@ -141,8 +141,8 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
   // results are the same.
   constexpr float kAbove = SHARED ? 0.f : kLazyRescale;
   [[maybe_unused]] constexpr float kBelow = kLazyRescale;
-  static_assert(!SHARED || SCORE != kScoreBias, "a shared tile's rows keep no distances");
-  constexpr bool LOG2 = SCORE != kScorePlain;  // scores in log2 units before the maxima, not raw products
+  static_assert(!SHARED || !score_biased(SCORE), "a shared tile's rows keep no distances");
+  constexpr bool LOG2 = score_capped(SCORE);  // scores in log2 units before the maxima, not raw products
   // This head dimension's query tiles per wave (in place of the namespace's).
   constexpr int kNT = prefill_nt<D>(), kQrowsPerWave = 16 * kNT;
   constexpr int kKeys = prefill_keys<D>();
@@ -318,7 +318,8 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
       qleft[nt] = a.window > 0 ? qpos[nt] - a.window + 1 : 0;
     }
     const uint16_t* src = a.query + (int64_t)batch_row * a.q_stride + (int64_t)(kvh * g + head) * D;
-    if constexpr (SCORE == kScoreBias) slope[nt] = qvalid[nt] ? a.slopes[kvh * g + head] * kLog2e : 0.f;
+    if constexpr (score_biased(SCORE))
+      slope[nt] = qvalid[nt] ? fminf(a.slopes[kvh * g + head], kMostSlope) * (LOG2 ? kLog2e : kLog2e / a.score_scale) : 0.f;
 #pragma unroll
     for (int c = 0; c < S::NC; ++c) {
       uint4 v = make_uint4(0, 0, 0, 0);
@@ -521,24 +522,32 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
   // scores (scale > 0), and p = exp2(fma(s, scale, -max)).
   auto softmax = [&](int tb) __attribute__((always_inline)) {
     const bool full = tb + kKeys - 1 <= wave_pos_min && tb >= wave_left_max;
-    if constexpr (!LOG2) mfma_results_ready(sc);
+    // With a distance bias the scores get its part inside the step (slope times
+    // the key's offset) here, one instruction each; the rest, the same for all of
+    // a lane's keys, joins the maximum and the exponent's base.
+    if constexpr (!LOG2 && SCORE != kScoreBias) mfma_results_ready(sc);
     // Mask, and each tile's row maximum over this lane's 4 kKG scores.
     float mx[kNT];
+    [[maybe_unused]] float bias0[kNT];
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
-      if constexpr (SCORE == kScoreCap) {
+      if constexpr (LOG2) {
 #pragma unroll
         for (int h = 0; h < kKG; ++h)
 #pragma unroll
           for (int r = 0; r < 4; ++r) sc[h][nt][r] = soft_cap(sc[h][nt][r] * a.score_scale, a.softcap_log2);
       }
+      if constexpr (SCORE == kScoreCapBias) {
+        const float distance = (float)(tb + 4 * q - qpos[nt]);
+#pragma unroll
+        for (int h = 0; h < kKG; ++h) sc[h][nt] += bias4(slope[nt], distance, h);
+      }
       if constexpr (SCORE == kScoreBias) {
-        f32x4_t column[kKG];
+        bias0[nt] = slope[nt] * (float)(tb + 4 * q - qpos[nt]);
 #pragma unroll
-        for (int h = 0; h < kKG; ++h) column[h] = sc[h][nt];
-        bias_scores(column, a.score_scale, a.softcap_log2, slope[nt], (float)(tb + 4 * q - qpos[nt]));
+        for (int h = 0; h < kKG; ++h)
 #pragma unroll
-        for (int h = 0; h < kKG; ++h) sc[h][nt] = column[h];
+          for (int r = 0; r < 4; ++r) sc[h][nt][r] = __builtin_fmaf(slope[nt], (float)(16 * h + r), sc[h][nt][r]);
       }
       if (!full) {
 #pragma unroll
@@ -553,6 +562,7 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
 #pragma unroll
       for (int i = 0; i < 4 * kKG; ++i) t[i] = sc[i >> 2][nt][i & 3];
       mx[nt] = tree_max(t);  // log2 units with softcap, raw scores without
+      if constexpr (SCORE == kScoreBias) mx[nt] += bias0[nt];
     }
     // The probabilities of both tiles are formed right away against the
     // running maxima, before the cross-lane reduction of the steps' maxima,
@@ -565,6 +575,7 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
     // 154.9 us against a branch per tile).
     auto probabilities = [&](int nt, float base) __attribute__((always_inline)) {
       float ps[4 * kKG];
+      if constexpr (SCORE == kScoreBias) base = __builtin_fmaf(-bias0[nt], a.score_scale, base);
 #pragma unroll
       for (int i = 0; i < 4 * kKG; ++i) {
         if constexpr (LOG2) ps[i] = fast_exp2(sc[i >> 2][nt][i & 3] - base);
@@ -602,6 +613,7 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
         if (!__builtin_amdgcn_ballot_w64(mx[nt] > (LOG2 ? m_run[nt] + kAbove : m_thr[nt]))) continue;
         float top = LOG2 ? mx[nt] : mx[nt] * a.score_scale;
         if constexpr (SHARED) top += kBelow;
+        if constexpr (SCORE == kScoreBias) top = base_above(top, bias0[nt] * a.score_scale);
         const float m_new = fmaxf(m_run[nt], top);
         const float alpha = m_run[nt] == -INFINITY ? 0.f : fast_exp2(m_run[nt] - m_new);
         m_run[nt] = m_new;
@@ -625,6 +637,14 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
   };
 
   static_assert(kStages == 2, "K and V alternate between two stages");
+  // The steps' keys ascend; with a distance bias they descend from the rows' own
+  // keys, where a positive slope leaves the largest scores: ascending, the
+  // maximum would rise by the slope's 64 keys at every step, and every step
+  // re-base (eight 512-row chunks on a 2048-token prefix, 32 heads' slopes from
+  // 0.84 to 2^-8: 214 us).
+  auto step_key = [&](int step) __attribute__((always_inline)) {
+    return kb0 + (score_biased(SCORE) ? nsteps - 1 - step : step) * kKeys;
+  };
   if constexpr (!kPingPong) {
     // One barrier per step: before it each wave waits for its own loads of
     // the current stage; after it every wave's loads of the stage have landed
@@ -633,11 +653,11 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
     // softmax, their LDS latency behind its arithmetic.
     Entries e_next{};
     {
-      const Offsets first = offsets_of(kb0, entry_of(kb0));
+      const Offsets first = offsets_of(step_key(0), entry_of(step_key(0)));
       issue(first, krs, kv[0][0]);
       issue(first, vrs, kv[0][1]);
     }
-    if (1 < nsteps) e_next = entry_of(kb0 + kKeys);
+    if (1 < nsteps) e_next = entry_of(step_key(1));
     if (__builtin_expect(div_group(wave * kQrowsPerWave) >= nr, 0)) {
       // All rows of this wave lie past the tile's last: it only loads its share
       // and keeps step, and the other wave of its SIMD has the matrix cores and
@@ -650,11 +670,11 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
         __syncthreads();
         wait_vmem_visible();
         if (step + 1 < nsteps) {
-          const int tb = kb0 + step * kKeys, next = (step + 1) & 1;
-          const Offsets of = offsets_of(tb + kKeys, e_next);
+          const int next = (step + 1) & 1;
+          const Offsets of = offsets_of(step_key(step + 1), e_next);
           issue(of, krs, kv[next][0]);
           issue(of, vrs, kv[next][1]);
-          if (step + 2 < nsteps) e_next = entry_of(tb + 2 * kKeys);
+          if (step + 2 < nsteps) e_next = entry_of(step_key(step + 2));
         }
       }
       return;
@@ -667,7 +687,7 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
     // to the direct-load asm as scalar words (make_rsrc).
     auto body = [&](int step, auto stage) __attribute__((always_inline)) {
       constexpr int cur = decltype(stage)::value, next = cur ^ 1;
-      const int tb = kb0 + step * kKeys;
+      const int tb = step_key(step);
       wait_vmem<0>();
       __syncthreads();
       // Every load of this wave has landed; tell the compiler. Its wait-count
@@ -678,10 +698,10 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
       // would then wait for (C4: 185.2 -> 183.9 us).
       wait_vmem_visible();
       if (step + 1 < nsteps) {
-        const Offsets of = offsets_of(tb + kKeys, e_next);
+        const Offsets of = offsets_of(step_key(step + 1), e_next);
         issue(of, krs, kv[next][0]);
         issue(of, vrs, kv[next][1]);
-        if (step + 2 < nsteps) e_next = entry_of(tb + 2 * kKeys);
+        if (step + 2 < nsteps) e_next = entry_of(step_key(step + 2));
       }
       scores(kv[cur][0]);
       if constexpr (D <= 128) {
@@ -726,22 +746,22 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
     // interval 2i + 1 (the first group's second barrier of the iteration, the
     // second group's first), after which the first group reads them.
     const bool lead = wave < kPrefillWaves / 2;
-    Entries e_next = entry_of(kb0);
-    Offsets off_v = offsets_of(kb0, e_next);  // offsets of the step whose V is issued next
+    Entries e_next = entry_of(step_key(0));
+    Offsets off_v = offsets_of(step_key(0), e_next);  // offsets of the step whose V is issued next
     issue(off_v, krs, kv[0][0]);
-    if (1 < nsteps) e_next = entry_of(kb0 + kKeys);
+    if (1 < nsteps) e_next = entry_of(step_key(1));
     wait_vmem<0>();
     __syncthreads();
     wait_vmem_visible();  // as in the other loop: the query (and entry) loads have landed
     if (!lead) __syncthreads();
     for (int i = 0; i <= nsteps; ++i) {
-      const int tb = kb0 + i * kKeys;
+      const int tb = step_key(i);
       if (i + 1 < nsteps) {
-        const Offsets off_k = offsets_of(tb + kKeys, e_next);
+        const Offsets off_k = offsets_of(step_key(i + 1), e_next);
         issue(off_k, krs, kv[(i + 1) & 1][0]);
         issue(off_v, vrs, kv[i & 1][1]);
         off_v = off_k;
-        if (i + 2 < nsteps) e_next = entry_of(tb + 2 * kKeys);
+        if (i + 2 < nsteps) e_next = entry_of(step_key(i + 2));
       } else if (i + 1 == nsteps) {
         issue(off_v, vrs, kv[i & 1][1]);
       }
