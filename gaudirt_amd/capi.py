@@ -103,8 +103,10 @@ class SharedPrefixList(_Sized):
     _fields_ = [
         ("struct_size", ctypes.c_size_t),
         ("words", c_void_p), ("row_request", c_void_p),
+        ("new_key", c_void_p), ("new_value", c_void_p), ("new_kv_row_stride", c_i64),
         ("part_cols", c_i64),
         ("rows", c_i32), ("tile_count", c_i32), ("workers", c_i32), ("worker_groups", c_i32), ("word_count", c_i32),
+        ("can_store", c_i32),
         ("map_at", c_i32), ("position_at", c_i32), ("merges_at", c_i32), ("tiles_at", c_i32), ("workers_at", c_i32),
         ("segments_at", c_i32),
     ]

@@ -90,10 +90,15 @@ struct PrefillArgs {
 struct SharedArgs : PrefillArgs {
   const int32_t* row_map;       // batch row of each compact row
   const int32_t* row_position;
-  const int32_t* worker_segs;   // [workers + 1] first segment of each worker
+  const int32_t* worker_list;   // SharedWorker records
   const int32_t* segs;          // SharedSegment records
   int32_t tile_count, workers;
   int64_t part_cols;            // columns of one kv head
+  // The new tokens' rows, which the workers then store (null: stored before).
+  const uint16_t* new_key;
+  const uint16_t* new_value;
+  int64_t new_stride;
+  uint16_t* pool_out;
 };
 
 template <int D>
@@ -201,7 +206,7 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
                  "s"(a.class_xcds), "s"(a.class_heads_div.mul), "s"(a.class_heads_div.shift), "s"(a.block_tables),
                  "s"(a.query), "s"(a.pool), "s"(a.group), "s"(a.bt_stride), "s"(a.block_shift), "s"(a.window),
                  "s"(a.q_stride), "s"(a.slots), "s"(a.kv_heads), "s"(a.group_div.mul), "s"(a.group_div.shift),
-                 "s"(a.row_map), "s"(a.row_position), "s"(a.tile_count), "s"(a.workers), "s"(a.worker_segs),
+                 "s"(a.row_map), "s"(a.row_position), "s"(a.tile_count), "s"(a.workers), "s"(a.worker_list),
                  "s"(a.segs));
     const int xcd = blockIdx.x % kXcds, j = blockIdx.x / kXcds;
     const int jl = (int)fast_div((uint32_t)j, a.class_heads_div);

@@ -170,14 +170,15 @@ int shared_prefix_list_build(const int32_t* run_first_row, const int32_t* run_ro
     };
     list->rows = (int32_t)plan.row_map.size();
     list->tile_count = (int32_t)plan.tiles.size();
-    list->workers = plan.worker_segs.empty() ? 0 : (int32_t)plan.worker_segs.size() - 1;
+    list->workers = (int32_t)plan.workers.size();
     list->worker_groups = plan.worker_groups;
     list->part_cols = plan.cols;
+    list->can_store = plan.stores;
     list->map_at = reserve(list->rows);
     list->position_at = reserve(list->rows);
     list->merges_at = reserve(int64_t{kSharedMergeWords} * list->rows);
     list->tiles_at = reserve(int64_t{kSharedTileWords} * list->tile_count);
-    list->workers_at = reserve((int64_t)plan.worker_segs.size());
+    list->workers_at = reserve(int64_t{kSharedWorkerWords} * list->workers);
     list->segments_at = reserve(int64_t{kSharedSegmentWords} * (int64_t)plan.segs.size());
     if (total > INT32_MAX) return bad("too much work");
     list->word_count = (int32_t)total;
@@ -191,7 +192,7 @@ int shared_prefix_list_build(const int32_t* run_first_row, const int32_t* run_ro
     put(list->position_at, plan.row_position);
     put(list->merges_at, plan.merges);
     put(list->tiles_at, plan.tiles);
-    put(list->workers_at, plan.worker_segs);
+    put(list->workers_at, plan.workers);
     put(list->segments_at, plan.segs);
     return GK_OK;
   } catch (const std::bad_alloc&) {
@@ -212,6 +213,13 @@ int shared_prefix_attention(const gk_prefill_params* p, const gk_shared_prefix_l
   if (list->rows == 0) return GK_OK;
   if (!list->words || !list->row_request || (reinterpret_cast<uintptr_t>(list->words) & 15))
     return fail(GK_ERR_INVALID_ARGUMENT, std::string(name) + ": null or misaligned list");
+  if (list->new_key) {
+    if (!list->can_store || !list->new_value)
+      return fail(GK_ERR_INVALID_ARGUMENT, std::string(name) + ": this list cannot store, or new_value is null");
+    if (int rc = check_kv_store(list->new_key, list->new_value, list->new_kv_row_stride, list->new_kv_row_stride, p->pool,
+                                p->kv_heads, p->head_dim))
+      return rc;
+  }
   const size_t need = workspace_bytes_of(p, list);
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))
     return fail(GK_ERR_WORKSPACE, std::string(name) + ": workspace too small or not 16-byte aligned (" +
@@ -222,11 +230,15 @@ int shared_prefix_attention(const gk_prefill_params* p, const gk_shared_prefix_l
   a.tile_count = list->tile_count;
   a.item_count = list->tile_count + list->worker_groups;
   a.workers = list->workers;
-  a.worker_segs = list->words + list->workers_at;
+  a.worker_list = list->words + list->workers_at;
   a.segs = list->words + list->segments_at;
   a.row_map = list->words + list->map_at;
   a.row_position = list->words + list->position_at;
   a.row_request = list->row_request;
+  a.new_key = static_cast<const uint16_t*>(list->new_key);
+  a.new_value = static_cast<const uint16_t*>(list->new_value);
+  a.new_stride = list->new_kv_row_stride;
+  a.pool_out = static_cast<uint16_t*>(const_cast<void*>(p->pool));
   a.part_cols = list->part_cols;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + output_bytes(p, list));

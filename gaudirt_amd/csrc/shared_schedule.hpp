@@ -13,6 +13,7 @@
 #pragma once
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <vector>
 
@@ -37,11 +38,21 @@ struct SharedTile {
 };
 constexpr int kSharedTileWords = 8;
 // A stretch of one worker's keys: `cols` columns of the compact rows from `first`
-// on, key tiles tile0 .. tile0 + tiles - 1.
+// on, key tiles tile0 .. tile0 + tiles - 1. pos >= 0: the rows are the batch rows
+// from batch_row on, at positions pos, pos + 1, ... (behind all of the segment's
+// keys, whatever they are, where no row's window starts among them); else they are
+// looked up. From key new_pos on, keys are the run's new tokens: those of the batch
+// rows from new_row on (INT32_MAX: none).
 struct SharedSegment {
-  int32_t first, cols, tile0, tiles, key_lo, key_hi, col, batch_row;
+  int32_t first, cols, tile0, tiles, key_lo, key_hi, col, batch_row, pos, new_pos, new_row, pad;
 };
-constexpr int kSharedSegmentWords = 8;
+constexpr int kSharedSegmentWords = 12;
+// A worker's first segment, and where its others stand among the segments.
+struct SharedWorker {
+  SharedSegment first;
+  int32_t next, end, pad[2];
+};
+constexpr int kSharedWorkerWords = 16;
 // Where a row's partials are: columns pre_col + p pre_stride (p < pre_parts) of
 // its prefix, own_col + p own_stride of its own keys, one column a head.
 struct SharedMerge {
@@ -50,32 +61,41 @@ struct SharedMerge {
 constexpr int kSharedMergeWords = 8;
 
 struct SharedPlan {
-  std::vector<int32_t> row_map, row_position, worker_segs;
+  std::vector<int32_t> row_map, row_position;
+  std::vector<SharedWorker> workers;
   std::vector<SharedMerge> merges;   // one per compact row
   std::vector<SharedTile> tiles;     // longest first
   std::vector<SharedSegment> segs;
   int64_t cols = 0;                  // partial columns of one kv head
   int32_t worker_groups = 0;         // workgroups of workers
+  bool stores = true;                // workers see every new token: they can store it
 };
 
-// What the split weighs, in microseconds.
+// What the split weighs, in microseconds. A worker's key tile takes `key_tile`
+// while few workers run; under load latency and bandwidth add up like the sides
+// of a right angle. Measured against the share of a kv head's CUs that workers
+// get, whole call (us): 64 rows of 32 to 1023 own keys behind 4096, 32 q / 8 kv
+// heads: 3 of 32 CUs 128, 8 65, 12 54, 16 49, 22 42, 27 39, 28 42; 256 rows of 16
+// to 700 behind 32000: 6 187, 8 177, 9 191, 16 212, 19 271; 48 rows of 16 q / 8
+// kv heads at head_dim 256 with a window: 8 243, 16 170, 22 145, 28 129.
 struct SharedCost {
   double step;        // a tile's step with all its waves busy, a quarter of it whatever the columns
   double tile_start;  // a workgroup's start and end
-  double key_tile;    // a worker's key tile where latency bounds it
+  double key_tile;    // a worker's key tile
   double bytes;       // of a worker's key tile
 };
 inline SharedCost shared_cost(int head_dim) {
-  if (head_dim == 64) return {0.6, 5.0, 1.8, 32 * 64 * 4.0};
-  if (head_dim == 128) return {1.7, 6.0, 2.2, 32 * 128 * 4.0};
-  return {1.3, 6.0, 2.2, 16 * 256 * 4.0};
+  if (head_dim == 64) return {0.65, 5.0, 1.8, 32 * 64 * 4.0};
+  if (head_dim == 128) return {1.95, 6.0, 2.35, 32 * 128 * 4.0};
+  return {1.8, 6.0, 2.35, 16 * 256 * 4.0};
 }
-constexpr double kSharedBandwidth = 5.8e6;  // bytes a microsecond that workers reach together
+constexpr double kSharedBandwidth = 6.3e6;  // bytes a microsecond
+constexpr double kSegmentTiles = 2.0;       // a segment's start and end, in key tiles
 
 // Work of one kv head before it is cut.
 struct SharedWork {
   int32_t first, rows, key_lo, key_hi;  // compact rows and their keys
-  bool own;                             // a run's own keys (else its group's prefix)
+  int32_t run;                          // compact row of the run whose own keys these are; -1: its group's prefix
   int32_t units;                        // steps of a tile, key tiles of a worker
   int32_t start;                        // first key, aligned
 };
@@ -87,15 +107,17 @@ inline SharedPlan shared_plan(const SharedRun* runs, int count, const int32_t* g
   const int step_keys = prefill_step_keys(head_dim), key_tile = shared_tile_keys(head_dim);
   const int columns = shared_columns(head_dim);
   std::vector<SharedWork> wide, narrow;
-  const auto add = [&](int first, int rows, int lo, int hi, bool own) {
+  const auto add = [&](int first, int rows, int lo, int hi, int run) {
     // Heads beyond a worker's columns go to a workgroup's tile; so do more than two workers' columns.
     if (lo >= hi) return;
-    SharedWork w{first, rows, lo, hi, own, 0, 0};
+    const bool own = run >= 0;
+    SharedWork w{first, rows, lo, hi, run, 0, 0};
     const bool tile = group > columns || rows * group > (own ? 2 * columns : columns);
     if (tile) {
       w.start = lo / step_keys * step_keys;
       w.units = (hi - w.start + step_keys - 1) / step_keys;
       wide.push_back(w);
+      plan.stores = plan.stores && !own;
       return;
     }
     const int most = columns / group;  // rows of a worker
@@ -121,7 +143,7 @@ inline SharedPlan shared_plan(const SharedRun* runs, int count, const int32_t* g
       }
       for (int r = 0; r < run.rows; r += tile_rows) {
         const int nr = std::min(tile_rows, run.rows - r), pos = run.pos + r;
-        add(at + r, nr, std::max(prefix, window > 0 ? pos - window + 1 : 0), pos + nr, true);
+        add(at + r, nr, std::max(prefix, window > 0 ? pos - window + 1 : 0), pos + nr, at);
       }
     }
     const int rows = (int)plan.row_map.size() - first;
@@ -132,33 +154,49 @@ inline SharedPlan shared_plan(const SharedRun* runs, int count, const int32_t* g
         lo = INT32_MAX;
         for (int k = 0; k < nr; ++k) lo = std::min(lo, std::max(0, plan.row_position[first + r + k] - window + 1));
       }
-      add(first + r, nr, lo, prefix, false);
+      add(first + r, nr, lo, prefix, -1);
     }
   }
+
+  // Pieces of at most `most` steps: the fewest steps with which one round of
+  // `room` workgroups holds all pieces; whole where there are more tiles than that.
+  const auto tile_pieces = [&](int room) {
+    int lo = 4, hi = 4;
+    for (const auto& w : wide) hi = std::max(hi, w.units);
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      int64_t sum = 0;
+      for (const auto& w : wide) sum += (w.units + mid - 1) / mid;
+      if (sum <= room) hi = mid;
+      else lo = mid + 1;
+    }
+    return lo;
+  };
 
   // How many of a kv head's CUs take workers: the number with which both kinds
   // of work, side by side, end soonest.
   const SharedCost cost = shared_cost(head_dim);
   const int slots = std::max(1, cus / kv_heads);
   int64_t key_tiles = 0;
-  double steps = 0;
-  int longest = 0;
   for (const auto& w : narrow) key_tiles += w.units;
-  const auto step_cost = [&](const SharedWork& w) {
-    const int waves = (w.rows * group + tile_cols / 8 - 1) / (tile_cols / 8);
-    return cost.step * (0.25 + 0.75 * waves / 8);
-  };
-  for (const auto& w : wide) {
-    steps += w.units * step_cost(w);
-    longest = std::max(longest, w.units);
-  }
   int best = narrow.empty() ? 0 : slots;
   if (!narrow.empty() && !wide.empty()) {
+    double steps = 0;
+    for (const auto& w : wide) {
+      const int waves = (w.rows * group + tile_cols / 8 - 1) / (tile_cols / 8);
+      steps = std::max(steps, cost.step * (0.25 + 0.75 * waves / 8));
+    }
+    const double bandwidth = key_tiles * cost.bytes * kv_heads / kSharedBandwidth;
     double best_time = 1e30;
-    for (int a = 1; a < slots || a == 1; ++a) {
-      const double rate = std::min(kSharedBandwidth, a * kv_heads * kSharedWaves * cost.bytes / cost.key_tile);
-      const double busy = key_tiles * cost.bytes * kv_heads / rate;
-      const double beside = steps / std::max(1, slots - a) + cost.tile_start;
+    const int stride = std::max(1, slots / 32);
+    for (int a = stride; a < slots || a == stride; a += stride) {
+      const double workers = double(a) * kSharedWaves;
+      const double latency = cost.key_tile * (key_tiles + kSegmentTiles * std::max<double>(workers, narrow.size())) / workers;
+      const double busy = std::sqrt(latency * latency + bandwidth * bandwidth);
+      const int room = std::max(1, slots - a), most = tile_pieces(room);
+      int64_t pieces = 0;
+      for (const auto& w : wide) pieces += (w.units + most - 1) / most;
+      const double beside = double((pieces + room - 1) / room) * (most * steps + cost.tile_start);
       const double time = std::max(busy, beside);
       if (time < best_time) {
         best_time = time;
@@ -179,28 +217,16 @@ inline SharedPlan shared_plan(const SharedRun* runs, int count, const int32_t* g
     for (int r = 0; r < w.rows; ++r) {
       SharedMerge& m = plan.merges[w.first + r];
       const int32_t at = (int32_t)(col + int64_t{r} * group);
-      if (w.own) m.own_col = at, m.own_parts = parts, m.own_stride = stride;
+      if (w.run >= 0) m.own_col = at, m.own_parts = parts, m.own_stride = stride;
       else m.pre_col = at, m.pre_parts = parts, m.pre_stride = stride;
     }
     return col;
   };
 
-  // Tiles: equal pieces of at most `most` steps, the fewest with which one round
-  // of workgroups holds all pieces; whole where there are more tiles than slots.
   if (!wide.empty()) {
-    int lo = 4, hi = std::max(4, longest);
-    const auto pieces = [&](int most) {
-      int64_t sum = 0;
-      for (const auto& w : wide) sum += (w.units + most - 1) / most;
-      return sum;
-    };
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (pieces(mid) <= tile_slots) hi = mid;
-      else lo = mid + 1;
-    }
+    const int most = tile_pieces(tile_slots);
     for (const auto& w : wide) {
-      const int parts = (w.units + lo - 1) / lo;
+      const int parts = (w.units + most - 1) / most;
       const int64_t col = place(w, parts);
       const int stride = (w.rows * group + 15) / 16 * 16;
       for (int p = 0, done = 0; p < parts; ++p) {
@@ -220,18 +246,18 @@ inline SharedPlan shared_plan(const SharedRun* runs, int count, const int32_t* g
   // for its start and end, in equal shares: the smallest with which the workers
   // suffice.
   if (workers) {
-    std::vector<int32_t> piece_ends, pieces_of;  // key tiles where each piece ends; pieces of each work
+    std::vector<int32_t> piece_ends, pieces_of, worker_segs;  // key tiles where each piece ends; pieces of each work
     int64_t share = std::max<int64_t>(3, (key_tiles + (int64_t)narrow.size() + workers - 1) / workers);
     for (;; share += std::max<int64_t>(1, share / 64)) {
       piece_ends.clear();
       pieces_of.clear();
-      plan.worker_segs.assign(1, 0);
+      worker_segs.assign(1, 0);
       int64_t room = share;
       for (const auto& w : narrow) {
         int pieces = 0;
         for (int done = 0; done < w.units; ++pieces) {
           if (room < 2) {
-            plan.worker_segs.push_back((int32_t)piece_ends.size());
+            worker_segs.push_back((int32_t)piece_ends.size());
             room = share;
           }
           int take = (int)std::min<int64_t>(w.units - done, room - 1);
@@ -242,21 +268,38 @@ inline SharedPlan shared_plan(const SharedRun* runs, int count, const int32_t* g
         }
         pieces_of.push_back(pieces);
       }
-      plan.worker_segs.push_back((int32_t)piece_ends.size());
-      if ((int)plan.worker_segs.size() - 1 <= workers) break;
+      worker_segs.push_back((int32_t)piece_ends.size());
+      if ((int)worker_segs.size() - 1 <= workers) break;
     }
-    size_t at = 0;
+    size_t at = 0, worker = 0;
     for (size_t i = 0; i < narrow.size(); ++i) {
       const SharedWork& w = narrow[i];
+      const int row0 = plan.row_map[w.first], pos0 = plan.row_position[w.first];
+      bool rows_follow = true, positions_follow = true;
+      for (int r = 1; r < w.rows; ++r) {
+        rows_follow = rows_follow && plan.row_map[w.first + r] == row0 + r;
+        positions_follow = positions_follow && plan.row_position[w.first + r] == pos0 + r;
+      }
+      const bool see_all = window <= 0 && w.run < 0;
+      const int pos = !rows_follow ? -1 : positions_follow ? pos0 : see_all ? w.key_hi : -1;
       const int64_t col = place(w, pieces_of[i]);
       const int stride = (w.rows * group + 15) / 16 * 16;
       for (int p = 0, done = 0; p < pieces_of[i]; ++p, ++at) {
-        plan.segs.push_back({w.first, w.rows * group, w.start / key_tile + done, piece_ends[at] - done, w.key_lo,
-                             w.key_hi, (int32_t)(col + int64_t{p} * stride), plan.row_map[w.first]});
+        const SharedSegment seg{w.first, w.rows * group, w.start / key_tile + done, piece_ends[at] - done, w.key_lo,
+                                w.key_hi, (int32_t)(col + int64_t{p} * stride), plan.row_map[w.first], pos,
+                                w.run < 0 ? INT32_MAX : plan.row_position[w.run],
+                                w.run < 0 ? 0 : plan.row_map[w.run], 0};
         done = piece_ends[at];
+        if ((int32_t)at == worker_segs[worker]) {
+          plan.workers.push_back({seg, (int32_t)plan.segs.size(), (int32_t)plan.segs.size(), {0, 0}});
+          ++worker;
+        } else {
+          plan.segs.push_back(seg);
+          plan.workers.back().end = (int32_t)plan.segs.size();
+        }
       }
     }
-    plan.worker_groups = ((int)plan.worker_segs.size() - 1 + kSharedWaves - 1) / kSharedWaves;
+    plan.worker_groups = ((int)plan.workers.size() + kSharedWaves - 1) / kSharedWaves;
   }
   return plan;
 }

@@ -22,21 +22,42 @@
 namespace gk {
 namespace {
 
-// 4 bytes per lane, HBM -> LDS (lds_dma16_w's narrow form).
-__device__ __forceinline__ void lds_dma4_w(uint32_t lds, u32x4_t rsrc, uint32_t voffset) {
+// lds_dma16_w for rows that one worker reads once (GK_KV_LOAD_POLICY).
+__device__ __forceinline__ void lds_dma16_once_w(uint32_t lds, u32x4_t rsrc, uint32_t voffset) {
   asm volatile(
       "s_mov_b32 m0, %0\n\t"
       "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen " GK_KV_LOAD_POLICY " lds" ::"s"(lds),
+      "v"(voffset), "s"(rsrc)
+      : "memory");
+}
+
+// 4 bytes per lane, HBM -> LDS (lds_dma16_w's narrow form; the s_nop also
+// covers a resource word that a readfirstlane has just made).
+__device__ __forceinline__ void lds_dma4_w(uint32_t lds, u32x4_t rsrc, uint32_t voffset) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 4\n\t"
       "buffer_load_dword %1, %2, 0 offen lds" ::"s"(lds),
       "v"(voffset), "s"(rsrc)
       : "memory");
 }
 
-// NT: 16-column tiles of the segment.
-template <int D, int SCORE, int NT>
-__device__ __forceinline__ void shared_segment(const SharedArgs& a, char* kt, int32_t* entries, int kvh, int first,
-                                               int ncols, int tile0, int ntiles, int key_lo, int key_hi, int64_t col,
-                                               const int32_t* bt) {
+// A segment's record (SharedSegment) in scalar registers.
+struct SegmentWords {
+  int first, ncols, tile0, ntiles, key_lo, key_hi, col, batch_row, pos, new_pos, new_row;
+};
+__device__ __forceinline__ SegmentWords load_segment(const int32_t* rec) {
+  return {scalar_load(rec, 0), scalar_load(rec, 1), scalar_load(rec, 2), scalar_load(rec, 3), scalar_load(rec, 4),
+          scalar_load(rec, 5), scalar_load(rec, 6), scalar_load(rec, 7), scalar_load(rec, 8), scalar_load(rec, 9),
+          scalar_load(rec, 10)};
+}
+
+// NT: 16-column tiles of the segment. `meanwhile` runs once its first loads are on their way.
+template <int D, int SCORE, int NT, class Meanwhile>
+__device__ __forceinline__ void shared_segment(const SharedArgs& a, char* kt, int32_t* entries, int kvh,
+                                               const SegmentWords& seg, const int32_t* bt, Meanwhile meanwhile) {
+  const int ncols = seg.ncols, tile0 = seg.tile0, ntiles = seg.ntiles, key_lo = seg.key_lo, key_hi = seg.key_hi;
   using S = MfmaShape<D>;
   constexpr bool LOG2 = SCORE != kScorePlain;
   constexpr int TS = S::TS, LOADS = S::LOADS, CPR = S::CPR;
@@ -66,7 +87,11 @@ __device__ __forceinline__ void shared_segment(const SharedArgs& a, char* kt, in
     const int j = nt * 16 + c16;
     const bool valid = j < ncols;
     const int row = (int)fast_div((uint32_t)min(j, ncols - 1), a.group_div), head = min(j, ncols - 1) - row * g;
-    const int batch_row = a.row_map[first + row], pos = a.row_position[first + row];
+    int batch_row = seg.batch_row + row, pos = seg.pos + row;
+    if (seg.pos < 0) {
+      batch_row = a.row_map[seg.first + row];
+      pos = a.row_position[seg.first + row];
+    }
     qpos[nt] = min(pos, key_end - 1);
     qleft[nt] = a.window > 0 ? max(key_begin, pos - a.window + 1) : key_begin;
     low = min(low, qpos[nt]);
@@ -80,6 +105,21 @@ __device__ __forceinline__ void shared_segment(const SharedArgs& a, char* kt, in
     }
   }
   const int pos_min = columns_min(low), left_max = -columns_min(-left);
+
+  // New tokens among the segment's keys: their rows come from the caller's
+  // tensors, not from the pool, where this wave stores them. Lanes 0 .. 2 CPR - 1
+  // (and again the lanes after them) hold the pieces of a token's key and value;
+  // those of the first new token are fetched ahead.
+  const int new_lo = max(key_begin, a.new_key ? seg.new_pos : INT32_MAX);
+  const bool key_lane = (lane & (2 * CPR - 1)) < CPR;
+  const int chunk = lane & (CPR - 1);
+  auto new_piece = [&](int key) __attribute__((always_inline)) {
+    const uint16_t* src = key_lane ? a.new_key : a.new_value;
+    return *reinterpret_cast<const u32x4_t*>(src + (int64_t)(seg.new_row + (key - seg.new_pos)) * a.new_stride +
+                                             (int64_t)kvh * D + chunk * 8);
+  };
+  u32x4_t ahead{0u, 0u, 0u, 0u};
+  if (new_lo < key_end) ahead = new_piece(new_lo);
 
   const uint32_t region = (uint32_t)(a.slots * D * 2);
   const uint16_t* kbase = a.pool + (int64_t)kvh * a.slots * D;
@@ -103,7 +143,7 @@ __device__ __forceinline__ void shared_segment(const SharedArgs& a, char* kt, in
   auto issue = [&](const Offsets& of, u32x4_t rs, char* tile) __attribute__((always_inline)) {
     const uint32_t base = lds_addr(tile);
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) lds_dma16_w(base + i * 1024, rs, of.v[i]);
+    for (int i = 0; i < LOADS; ++i) lds_dma16_once_w(base + i * 1024, rs, of.v[i]);
   };
 
   f32x4_t o[NT][S::NO];
@@ -124,11 +164,28 @@ __device__ __forceinline__ void shared_segment(const SharedArgs& a, char* kt, in
   Offsets next = offsets_of(tile0);
   issue(next, krs, kt);
   issue(next, vrs, vt);
+  meanwhile();
   for (int t = tile0; t < tile_end; ++t) {
     const int tb = t * TS;
     const bool more = t + 1 < tile_end;
     // In flight: (entries of t + 1,) K, V of t, in this order.
-    wait_vmem<LOADS>();
+    if (tb + TS > new_lo && new_lo < key_end) {
+      wait_vmem<0>();
+      for (int key = max(tb, new_lo); key < min(tb + TS, key_end); ++key) {
+        u32x4_t v = ahead;
+        if (key != new_lo) v = new_piece(key);
+        const int tt = key - tb;
+        *reinterpret_cast<u32x4_t*>(kt + (key_lane ? 0 : S::TILE) + tt * (2 * D) + ((chunk ^ swz(tt, D / 8)) << 4)) = v;
+        const int32_t entry = entries[(t & 1) * kWorkerEntries + tt];
+        const int64_t slot = ((int64_t)entry << shift) | (key & bmask);
+        if (entry >= 0 && slot < a.slots && lane < 2 * CPR)
+          __builtin_nontemporal_store(v, reinterpret_cast<u32x4_t*>(
+                                             a.pool_out + ((int64_t)(key_lane ? kvh : a.kv_heads + kvh) * a.slots + slot) * D + chunk * 8));
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    } else {
+      wait_vmem<LOADS>();
+    }
     bf16x8_t kr[S::TG][S::NC];
 #pragma unroll
     for (int h = 0; h < S::TG; ++h) {
@@ -266,7 +323,7 @@ __device__ __forceinline__ void shared_segment(const SharedArgs& a, char* kt, in
   }
 
   // The partial: unnormalised rows of head_dim floats, (base, sum) beside them.
-  const int64_t col0 = (int64_t)kvh * a.part_cols + col;
+  const int64_t col0 = (int64_t)kvh * a.part_cols + seg.col;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const float l = col4_sum(l_run[nt]);
@@ -291,18 +348,24 @@ __device__ __forceinline__ void shared_worker(const SharedArgs& a, char* lds, in
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   char* kt = lds + wave * (2 * S::TILE);
   int32_t* entries = reinterpret_cast<int32_t*>(lds + kSharedWaves * 2 * S::TILE) + wave * 2 * kWorkerEntries;
-  const int s1 = scalar_load(a.worker_segs, worker + 1);
-  for (int s = scalar_load(a.worker_segs, worker); s < s1; ++s) {
-    const int32_t* rec = a.segs + (int64_t)s * kSharedSegmentWords;
-    const int first = scalar_load(rec, 0), ncols = scalar_load(rec, 1), tile0 = scalar_load(rec, 2),
-              ntiles = scalar_load(rec, 3), key_lo = scalar_load(rec, 4), key_hi = scalar_load(rec, 5),
-              col = scalar_load(rec, 6), request = scalar_load(a.row_request, scalar_load(rec, 7));
+  // The next segment's record, and the request behind it, come while a segment runs.
+  const int32_t* rec = a.worker_list + (int64_t)worker * kSharedWorkerWords;
+  SegmentWords seg = load_segment(rec), next;
+  int at = scalar_load(rec, kSharedSegmentWords), request = scalar_load(a.row_request, seg.batch_row), next_request = 0;
+  const int end = scalar_load(rec, kSharedSegmentWords + 1);
+  for (;;) {
+    const bool more = at < end;
+    next = more ? load_segment(a.segs + (int64_t)at * kSharedSegmentWords) : seg;
+    const auto meanwhile = [&] { next_request = scalar_load(a.row_request, next.batch_row); };
     const int32_t* bt = a.block_tables + (int64_t)request * a.bt_stride;
-    if (shared_columns(D) == 16 || ncols <= 16)
-      shared_segment<D, SCORE, 1>(a, kt, entries, kvh, first, ncols, tile0, ntiles, key_lo, key_hi, col, bt);
+    if (shared_columns(D) == 16 || seg.ncols <= 16)
+      shared_segment<D, SCORE, 1>(a, kt, entries, kvh, seg, bt, meanwhile);
     else
-      shared_segment<D, SCORE, shared_columns(D) / 16>(a, kt, entries, kvh, first, ncols, tile0, ntiles, key_lo, key_hi,
-                                                       col, bt);
+      shared_segment<D, SCORE, shared_columns(D) / 16>(a, kt, entries, kvh, seg, bt, meanwhile);
+    if (!more) return;
+    seg = next;
+    request = next_request;
+    ++at;
   }
 }
 

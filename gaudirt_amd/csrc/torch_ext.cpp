@@ -36,6 +36,7 @@
 #include <mutex>
 #include <numeric>
 #include <unordered_map>
+#include <unordered_set>
 #include <utility>
 #include <vector>
 
@@ -284,6 +285,8 @@ struct SharedPrefixPlan {
   int64_t prefill_uncut_offset = 0;
   int32_t prefill_uncut_items = 0;
   at::Tensor row_request;
+  bool stores = false;     // the new tokens are stored along the way
+  bool by_itself = false;  // every row attends by itself: paged_attn's own path
 };
 
 // ---------------------------------------------------------------------------
@@ -880,7 +883,8 @@ class PagedMetadata : public torch::CustomClassHolder {
     if (cached != shared_plans_.end()) return cached->second;
     check_groups(group_rows, group_prefix);
     SharedPrefixPlan plan;
-    if (query_heads / kv_heads > 128) return shared_plans_.emplace(std::move(key), std::move(plan)).first->second;
+    plan.by_itself = query_heads / kv_heads > 128 || attends_in_one_launch(query_heads, kv_heads, head_dim, window);
+    if (plan.by_itself) return shared_plans_.emplace(std::move(key), std::move(plan)).first->second;
     const int group = static_cast<int>(query_heads / kv_heads);
     const int64_t tile_rows = std::max<int64_t>(1, gk::prefill_tile_qrows(static_cast<int>(head_dim)) / group);
     // Runs, cut where groups meet. A run that fills a tile of the prefill kernel
@@ -888,11 +892,17 @@ class PagedMetadata : public torch::CustomClassHolder {
     // from its group.
     std::vector<int32_t> first, rows, pos, of_group, prefix(group_prefix.begin(), group_prefix.end());
     std::vector<int32_t> chunk_first, chunk_rows, chunk_pos;
-    int64_t g = 0, group_end = group_rows.empty() ? 0 : group_rows[0];
+    int64_t g = 0, group_end = group_rows[0];
+    // A host request map says which rows are one request's. Where each request is
+    // one run, nobody but the run's own rows sees its new tokens.
+    std::unordered_set<int32_t> seen;
+    plan.stores = !mapping_h_.empty();
     for (const auto& run : sequences_) {
+      if (plan.stores) plan.stores = seen.insert(requests_h_[run.row]).second;
       for (int64_t r = run.row; r < run.row + run.length;) {
         while (r >= group_end) group_end += group_rows[++g];
         const int64_t end = std::min<int64_t>(run.row + run.length, group_end);
+        plan.stores = plan.stores && end - r == run.length;
         const bool chunk = end - r >= tile_rows;
         (chunk ? chunk_first : first).push_back(static_cast<int32_t>(r));
         (chunk ? chunk_rows : rows).push_back(static_cast<int32_t>(end - r));
@@ -925,6 +935,8 @@ class PagedMetadata : public torch::CustomClassHolder {
       }
       append(work);
     }
+    plan.stores = plan.stores && chunk_rows.empty() && plan.shared.can_store;
+    plan.by_itself = rows.empty();
     int64_t items_at = 0, merges_at = 0;
     if (!chunk_rows.empty()) {
       const auto build = [&](auto list_build, gk_prefill_list& list) {
@@ -955,6 +967,34 @@ class PagedMetadata : public torch::CustomClassHolder {
   struct Sequence {
     int32_t row, length, prefix;
   };
+
+  // Short batches take one launch row by row (the decode kernel with a workgroup a
+  // unit), three or two here; where both sides read about as much, that decides.
+  // Measured (us, row by row / shared; 200 own tokens at most): 32 q / 8 kv heads,
+  // 32 rows behind 512 tokens 12.8 / 19.1 (84 MB row by row), 64 behind 256 16.1 /
+  // 21.6 (99 MB), 16 behind 1024 14.9 / 19.3, 32 behind 1024 15.9 / 18.9 (151 MB),
+  // 64 behind 512 22.8 / 23.1 (166 MB); 8 q / 2 kv heads, 64 rows of 1000 own
+  // tokens behind 512 18.6 / 20.7 (84 MB), behind 1024 22.7 / 21.0 (118 MB).
+  // Beyond that kernel's contexts sharing gains from about 30 MB on, and loses less
+  // than 1 us below: 4 rows behind 2048 17.0 / 17.1, 8 behind 4096 29.0 / 22.4.
+  bool attends_in_one_launch(int64_t query_heads, int64_t kv_heads, int64_t head_dim, int64_t window) const {
+    gk_decode_params p{};
+    p.struct_size = sizeof(p);
+    p.rows = static_cast<int32_t>(rows_);
+    p.q_heads = static_cast<int32_t>(query_heads);
+    p.kv_heads = static_cast<int32_t>(kv_heads);
+    p.head_dim = static_cast<int32_t>(head_dim);
+    p.block_size = static_cast<int32_t>(page_);
+    p.sliding_window = static_cast<int32_t>(window);
+    int64_t keys = 0;
+    for (const auto& run : sequences_) {
+      if (run.length >= kPrefillMinRows) return false;
+      const int64_t context = run.prefix + run.length;
+      p.max_context = static_cast<int32_t>(std::max<int64_t>(p.max_context, context));
+      keys += run.length * (window > 0 ? std::min(window, context) : context);
+    }
+    return keys * kv_heads * head_dim * 4 <= (int64_t{100} << 20) && gk_paged_decode_schedule(&p) == GK_DECODE_UNIT;
+  }
 
   void check_groups(const std::vector<int64_t>& group_rows, const std::vector<int64_t>& group_prefix) const {
     TORCH_CHECK(!group_rows.empty() && group_rows.size() == group_prefix.size(),
@@ -1339,9 +1379,9 @@ at::Tensor shared_prefix_attn(const at::Tensor& query, const at::Tensor& key, co
   check_attention(plan, query, key, value, key_pool, value_pool, locations, head_dim, scale, softcap, sliding_window);
   const auto& work = metadata->shared_prefix_plan(group_rows, group_prefix, plan.query_heads, plan.kv_heads, head_dim,
                                                   sliding_window);
-  // Batch-invariant calls attend every row by itself, and so do groups of more
-  // than 128 query heads a kv head, which fill the decode kernels alone.
-  if (g_decode_partition.load(std::memory_order_relaxed) > 0 || !work.shared.rows)
+  // Batch-invariant calls attend every row by itself, and so do short batches and
+  // more than 128 query heads a kv head, which fill the decode kernels alone.
+  if (g_decode_partition.load(std::memory_order_relaxed) > 0 || work.by_itself)
     return paged_attn_impl(query, key, value, key_pool, value_pool, locations, plan_tensor, head_dim, scale, softcap,
                            sliding_window, nullptr);
   const hipStream_t stream = current_stream();
@@ -1349,15 +1389,22 @@ at::Tensor shared_prefix_attn(const at::Tensor& query, const at::Tensor& key, co
   const auto q = kernel_rows(query), k = kernel_rows(key), v = kernel_rows(value);
   auto output = bucket_output(query, plan.rows, query.size(1));
   void* pool = key_pool.data_ptr();
-  check_gk(gk_kv_store(k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), locations.data_ptr<int32_t>(),
-                       static_cast<int32_t>(plan.rows), pool, plan.slots, static_cast<int32_t>(plan.kv_heads),
-                       static_cast<int32_t>(head_dim), stream),
-           "GaudiRT attention: KV store");
+  auto list = work.shared;
+  if (work.stores && k.stride(0) == v.stride(0)) {
+    list.new_key = k.data_ptr();
+    list.new_value = v.data_ptr();
+    list.new_kv_row_stride = k.stride(0);
+  } else {
+    check_gk(gk_kv_store(k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), locations.data_ptr<int32_t>(),
+                         static_cast<int32_t>(plan.rows), pool, plan.slots, static_cast<int32_t>(plan.kv_heads),
+                         static_cast<int32_t>(head_dim), stream),
+             "GaudiRT attention: KV store");
+  }
   const auto params = prefill_params(plan, q, pool, output, static_cast<float>(scale), static_cast<float>(softcap),
                                      sliding_window);
-  const size_t need = gk_shared_prefix_workspace_bytes(&params, &work.shared);
+  const size_t need = gk_shared_prefix_workspace_bytes(&params, &list);
   const auto workspace = at::empty({static_cast<int64_t>(need)}, query.options().dtype(at::kByte));
-  check_gk(gk_shared_prefix_attention(&params, &work.shared, workspace.data_ptr(), need, stream),
+  check_gk(gk_shared_prefix_attention(&params, &list, workspace.data_ptr(), need, stream),
            "GaudiRT shared-prefix attention");
   if (work.prefill.item_count)
     launch_prefill_list(params, work.prefill, work.words.data_ptr<int32_t>() + work.prefill_uncut_offset,

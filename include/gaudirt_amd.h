@@ -254,18 +254,24 @@ int gk_paged_prefill_alibi(const gk_prefill_params* params, const gk_prefill_lis
  * it fills `list` but for its two pointers and writes word_count words
  * (GK_ERR_WORKSPACE, with word_count set, when capacity is smaller). The caller
  * copies the words to the device, 16-byte aligned, and sets words to the copy
- * and row_request to the block-table row of every batch row (device).
+ * and row_request to the block-table row of every batch row (device). The new
+ * tokens are in the pool before the call or, where the list says can_store and
+ * every request of the batch is one run of the list, ride along: new_key and
+ * new_value hold their rows (batch rows, as gk_kv_store takes them), which the
+ * call attends and stores at the slots of their positions.
  * gk_shared_prefix_attention does not read seq_*, seqs and max_rows of its
  * gk_prefill_params and writes the list's rows only; its sliding_window is the
- * list's. Every key, the rows' own included, is in the pool (store first).
- * A GQA group of at most 128; at most 65535 rows.
+ * list's. A GQA group of at most 128; at most 65535 rows.
  * ------------------------------------------------------------------------- */
 typedef struct gk_shared_prefix_list {
   size_t struct_size;          /* sizeof(gk_shared_prefix_list) as the caller was built; checked */
   const int32_t* words;
   const int32_t* row_request;
+  const void* new_key;         /* bf16 [batch rows, new_kv_row_stride], or NULL: stored before */
+  const void* new_value;
+  int64_t new_kv_row_stride;
   int64_t part_cols;           /* partial results of one kv head */
-  int32_t rows, tile_count, workers, worker_groups, word_count;
+  int32_t rows, tile_count, workers, worker_groups, word_count, can_store;
   int32_t map_at, position_at, merges_at, tiles_at, workers_at, segments_at;  /* sections of the words */
 } gk_shared_prefix_list;
 

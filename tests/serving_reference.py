@@ -15,12 +15,14 @@ and 2^-23 of a bias; a weight is off by e times that, twice for the sum. Every
 term is computed from the case itself.
 """
 
+import ctypes
 import math
 
 import numpy as np
 import torch
 
 import gaudirt_amd
+from gaudirt_amd import capi
 
 
 class Batch:
@@ -145,3 +147,48 @@ class Batch:
 
 def same_bits(a, b):
     return torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+def shared_prefix_c(b, softcap=0.0, window=-1, ride_along=False, page=None):
+    """The batch through gk_shared_prefix_list_build and gk_shared_prefix_attention, whatever its size (the operator
+    lets short batches attend row by row): the new rows stored by gk_kv_store first, or with ride_along by the call
+    itself. Rows of the output that the call does not write are NaN."""
+    lib, page = capi.load(), page or b.page
+    as_i32 = lambda a: np.ascontiguousarray(a, dtype=np.int32)  # noqa: E731
+    news = as_i32([n for _, _, n in b.requests])
+    first = as_i32(np.concatenate([[0], np.cumsum(news)[:-1]]))
+    pos = as_i32([b.prefix[g] + own for g, own, _ in b.requests])
+    group, prefix = as_i32([g for g, _, _ in b.requests]), as_i32(b.group_prefix)
+    host = lambda a: ctypes.c_void_p(a.ctypes.data)  # noqa: E731
+    words, lst = np.zeros(1 << 20, dtype=np.int32), capi.SharedPrefixList()
+    capi.check(lib.gk_shared_prefix_list_build(host(first), host(news), host(pos), host(group), len(news), host(prefix),
+                                               len(prefix), b.q_heads, b.kv_heads, b.d, window, host(words), words.size,
+                                               ctypes.byref(lst)))
+    device_words = torch.from_numpy(words[:lst.word_count].copy()).cuda()
+    row_request = torch.from_numpy(as_i32(b.row_request)).cuda()
+    tables = b.mapping[:, ::page].copy()
+    tables[tables >= 0] //= page
+    tables = torch.from_numpy(tables).cuda()
+    locations = torch.from_numpy(as_i32(b.locations)).cuda()
+    out = torch.full((b.rows, b.q_heads * b.d), float("nan"), dtype=torch.bfloat16, device="cuda")
+    lst.words, lst.row_request = device_words.data_ptr(), row_request.data_ptr()
+    if ride_along:
+        assert lst.can_store
+        lst.new_key, lst.new_value, lst.new_kv_row_stride = b.key.data_ptr(), b.value.data_ptr(), b.key.stride(0)
+    else:
+        capi.check(lib.gk_kv_store(capi.ptr(b.key), capi.ptr(b.value), b.key.stride(0), b.value.stride(0),
+                                   capi.ptr(locations), b.rows, capi.ptr(b.pool), b.slots, b.kv_heads, b.d,
+                                   capi.current_stream()))
+    p = capi.PrefillParams()
+    p.query, p.q_row_stride = b.query.data_ptr(), b.query.stride(0)
+    p.pool, p.slots = b.pool.data_ptr(), b.slots
+    p.block_tables, p.bt_stride, p.block_size = tables.data_ptr(), tables.stride(0), page
+    p.q_heads, p.kv_heads, p.head_dim = b.q_heads, b.kv_heads, b.d
+    p.scale, p.softcap, p.sliding_window = b.scale, softcap, window
+    p.out, p.out_row_stride = out.data_ptr(), out.stride(0)
+    need = lib.gk_shared_prefix_workspace_bytes(ctypes.byref(p), ctypes.byref(lst))
+    workspace = torch.full((need // 4 + 64,), float("nan"), device="cuda")  # a word past `need` must stay as it is
+    capi.check(lib.gk_shared_prefix_attention(ctypes.byref(p), ctypes.byref(lst), capi.ptr(workspace), need,
+                                              capi.current_stream()))
+    assert torch.isnan(workspace[need // 4:]).all(), "the workspace was left"
+    return out, bool(lst.can_store)

@@ -55,22 +55,38 @@ void check(const std::vector<gk::SharedRun>& runs, const std::vector<int32_t>& p
     expect(i == 0 || plan.tiles[i - 1].steps >= t.steps, "tiles are not longest first", trial);
     add(t.first, t.rows, std::max(t.key_lo, t.key0), std::min(t.key_hi, t.key0 + t.steps * step), t.col, t.batch_row);
   }
-  size_t at = 0;
-  for (const auto& s : plan.segs) {
+  const auto segment = [&](const gk::SharedSegment& s) {
     expect(s.tiles > 0 && s.cols > 0 && s.cols <= gk::shared_columns(d) && s.cols % group == 0, "a segment", trial);
     add(s.first, s.cols / group, std::max(s.key_lo, s.tile0 * tile), std::min(s.key_hi, (s.tile0 + s.tiles) * tile), s.col,
         s.batch_row);
+    // New tokens: the run's rows, seen by a run's own segments only.
+    if (s.new_pos != INT32_MAX) {
+      const gk::SharedRun* run = nullptr;
+      for (const auto& x : runs)
+        if (s.batch_row >= x.first_row && s.batch_row < x.first_row + x.rows) run = &x;
+      expect(run && s.new_pos == run->pos && s.new_row == run->first_row && s.key_hi <= run->pos + run->rows &&
+                 s.key_lo >= std::min(prefix[run->group], run->pos),
+             "a segment's new tokens", trial);
+    } else {
+      expect(s.key_hi <= prefix[row_run[s.first].group], "an own segment without its new tokens", trial);
+    }
+    if (s.pos < 0) return;
+    for (int r = 0; r < s.cols / group && s.first + r < (int)rows; ++r) {
+      const int pos = row_run[s.first + r].pos;
+      expect(plan.row_map[s.first + r] == s.batch_row + r, "a segment's rows do not follow each other", trial);
+      expect(s.pos + r == pos || (window <= 0 && std::min(s.pos + r, pos) >= s.key_hi - 1), "a segment's positions", trial);
+    }
+  };
+  int32_t at = 0;
+  for (const auto& w : plan.workers) {
+    expect(w.next == at && w.end >= w.next, "a worker's segments", trial);
+    segment(w.first);
+    for (at = w.next; at < w.end && at < (int32_t)plan.segs.size(); ++at) segment(plan.segs[at]);
   }
-  if (!plan.worker_segs.empty()) {
-    expect(plan.worker_segs.front() == 0 && plan.worker_segs.back() == (int32_t)plan.segs.size(), "worker ends", trial);
-    for (at = 1; at < plan.worker_segs.size(); ++at)
-      expect(plan.worker_segs[at] > plan.worker_segs[at - 1], "a worker without work", trial);
-    expect(((int)plan.worker_segs.size() - 1 + 7) / 8 == plan.worker_groups, "worker groups", trial);
-    if (plan.tiles.empty())
-      expect(plan.worker_groups <= std::max(1, 256 / kv_heads), "more workers than fit the GPU at once", trial);
-  } else {
-    expect(plan.segs.empty() && plan.worker_groups == 0, "segments without workers", trial);
-  }
+  expect(at == (int32_t)plan.segs.size(), "segments without a worker", trial);
+  expect(((int)plan.workers.size() + 7) / 8 == plan.worker_groups, "worker groups", trial);
+  if (plan.tiles.empty())
+    expect(plan.worker_groups <= std::max(1, 256 / kv_heads), "more workers than fit the GPU at once", trial);
   // Every row: its visible keys, each once.
   size_t named = 0;
   for (size_t i = 0; i < rows; ++i) {

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import gaudirt_amd
-from tests.serving_reference import Batch, same_bits
+from tests.serving_reference import Batch, same_bits, shared_prefix_c
 
 pytestmark = pytest.mark.gpu
 
@@ -24,10 +24,21 @@ def run(b, group_rows=None, group_prefix=None, softcap=0.0, window=-1, **kw):
 
 
 def check(b, **kind):
-    expected_pool = b.stored()
+    """The operator, and the C entry with the new rows stored first and along the way: the operator lets short
+    batches attend row by row."""
+    before, expected_pool = b.pool.clone(), b.stored()
     out = run(b, **kind)
     b.check(out, **kind)
     assert same_bits(b.pool, expected_pool), "pool bytes differ"
+    if b.q_heads // b.kv_heads <= 128:
+        b.pool.copy_(before)
+        stored, can_store = shared_prefix_c(b, **kind)
+        b.check(stored, **kind)
+        assert same_bits(b.pool, expected_pool)
+        if can_store:
+            b.pool.copy_(before)
+            along, _ = shared_prefix_c(b, ride_along=True, **kind)
+            assert same_bits(along, stored) and same_bits(b.pool, expected_pool), "rows stored along the way"
     return out
 
 
@@ -84,6 +95,45 @@ def test_declared_shorter_than_shared():
     b = Batch(9, decode(2, 8, 100), [640, 320])
     for prefix in ([0, 0], [1, 319], [33, 64], [640, 320]):
         b.check(run(b, group_prefix=prefix))
+        b.group_prefix = prefix
+        check(b)
+
+
+def test_long_batches_share_through_the_operator():
+    # Contexts beyond the one-launch decode kernel's: shared whatever the bytes; host and device metadata.
+    for kind in ("host", "device", "scheduler"):
+        b = Batch(30, decode(1, 20, 300) + [(1, 4, 5), (1, 9, 1)], [4000, 2600], metadata=kind)
+        out = check(b)
+        assert same_bits(out, shared_prefix_c(b)[0])
+
+
+def test_rows_of_one_request_in_two_runs():
+    # One request's chunk in two groups: the second part's rows see the first part's new keys.
+    b = Batch(31, [(0, 5, 6), (0, 9, 1), (0, 11, 1)], [2400], heads=(8, 2, 128))
+    expected, bound = b.attend()
+    out = run(b, group_rows=[4, 4], group_prefix=[b.group_prefix[0], 16])
+    assert bool(((out.double() - expected).abs() <= bound).all())
+    assert same_bits(b.pool, b.stored())
+    # The same rows, the request's later part first.
+    order = [4, 5, 0, 1, 2, 3, 6, 7]
+    for name in ("query", "key", "value"):
+        setattr(b, name, getattr(b, name)[order].contiguous())
+    b.locations, b.row_request, b.positions = b.locations[order], b.row_request[order], b.positions[order]
+    b.pool.normal_()
+    b.metadata = b.make_metadata()
+    pool, sequential = b.stored(), []
+    out = run(b, group_rows=[8], group_prefix=[b.group_prefix[0]])
+    assert same_bits(b.pool, pool)
+    for row in range(8):  # each row against plain attention over the stored pool
+        n, group = int(b.positions[row]) + 1, b.q_heads // b.kv_heads
+        at = torch.from_numpy(b.mapping[b.row_request[row], :n]).cuda().long()
+        for h in range(b.q_heads):
+            q = b.query[row].view(b.q_heads, b.d)[h].double()
+            weight = torch.softmax(pool[0, 0, h // group][at].double() @ q * b.scale, 0)
+            value = pool[0, 1, h // group][at].double()
+            limit = 2.0 ** -8 * (2 * (weight @ value.abs()) + (weight @ value).abs()) * 1.02 + 1e-3 * (weight @ value.abs())
+            sequential.append(bool(((out[row].view(b.q_heads, b.d)[h].double() - weight @ value).abs() <= limit).all()))
+    assert all(sequential)
 
 
 def test_many_groups():
@@ -107,24 +157,24 @@ def test_extreme_values():
     b = Batch(15, decode(2, 9, 200), [300, 128], value_scale=1e37)
     b.query *= 300.0
     b.value *= 1e37
-    out = run(b)
-    assert torch.isfinite(out).all()
     exact, _ = b.attend()
-    assert float(((out.double() - exact).abs() / exact.abs().max()).max()) < 2.0 ** -6
+    for out in (run(b), shared_prefix_c(b)[0]):
+        assert torch.isfinite(out).all()
+        assert float(((out.double() - exact).abs() / exact.abs().max()).max()) < 2.0 ** -6
 
 
 def test_other_rows_infinities_stay_theirs():
     b = Batch(16, decode(1, 6, 80), [160], heads=(8, 2, 128))
     exact, _ = b.attend()
     b.key[2], b.value[2] = float("nan"), float("inf")
-    out = run(b)
     others = [i for i in range(b.rows) if i != 2]
-    assert torch.isfinite(out[others]).all() and not torch.isfinite(out[2]).all()
-    assert float((out.double() - exact)[others].abs().max()) < 0.05
+    for out in (run(b), shared_prefix_c(b)[0], shared_prefix_c(b, ride_along=True)[0]):
+        assert torch.isfinite(out[others]).all() and not torch.isfinite(out[2]).all()
+        assert float((out.double() - exact)[others].abs().max()) < 0.05
 
 
 def test_batch_invariant_mode_attends_row_by_row():
-    b = Batch(17, decode(2, 9, 300), [513, 200])
+    b = Batch(17, decode(2, 9, 300), [2513, 200])
     gaudirt_amd.set_batch_invariant_decode(True)
     try:
         out = run(b)
@@ -136,9 +186,9 @@ def test_batch_invariant_mode_attends_row_by_row():
 
 
 def test_repeats_and_layers_give_the_same_bits():
-    b = Batch(18, decode(2, 20, 300) + [(1, 3, 9)], [513, 800])
+    b = Batch(18, decode(2, 20, 300) + [(1, 3, 9)], [513, 2800])
     first = run(b)
-    second = Batch(19, decode(1, 30, 100), [640])
+    second = Batch(19, decode(1, 30, 100), [2640])
     for _ in range(5):
         run(second)
         assert same_bits(run(b), first)
@@ -146,7 +196,7 @@ def test_repeats_and_layers_give_the_same_bits():
 
 
 def test_strided_and_misaligned_inputs():
-    b = Batch(20, decode(2, 9, 300), [513, 200])
+    b = Batch(20, decode(2, 9, 300), [2513, 200])
     expected = run(b)
     wide = torch.zeros(b.rows, b.query.shape[1] + 24, dtype=torch.bfloat16, device="cuda")
     for offset in (0, 8, 3):
@@ -158,7 +208,7 @@ def test_strided_and_misaligned_inputs():
 
 
 def test_another_stream():
-    b = Batch(21, decode(2, 9, 300), [513, 200])
+    b = Batch(21, decode(2, 9, 300), [2513, 200])
     expected = run(b)
     torch.cuda.synchronize()
     side = torch.cuda.Stream()
@@ -172,7 +222,7 @@ def test_another_stream():
 
 
 def test_two_streams_at_once():
-    batches = [Batch(22 + i, decode(2, 20, 400), [2048, 1024]) for i in range(2)]
+    batches = [Batch(22 + i, decode(2, 20, 400), [2048, 2400]) for i in range(2)]
     expected = [run(b) for b in batches]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in batches]
@@ -193,8 +243,8 @@ def test_two_streams_at_once():
 
 
 def test_captured_and_replayed():
-    b = Batch(24, decode(2, 12, 300), [513, 800])
-    other = Batch(25, decode(1, 20, 100), [640])
+    b = Batch(24, decode(2, 12, 300), [513, 2800])
+    other = Batch(25, decode(1, 20, 100) + [(0, 3, 40)], [2640])
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
