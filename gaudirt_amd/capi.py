@@ -236,7 +236,7 @@ def load():
     lib.gk_paged_decode_alibi.argtypes = [ctypes.POINTER(DecodeParams), c_void_p, c_void_p, ctypes.c_size_t, c_void_p]
     lib.gk_paged_prefill_alibi.argtypes = [ctypes.POINTER(PrefillParams), ctypes.POINTER(PrefillList), c_void_p,
                                            c_void_p, ctypes.c_size_t, c_void_p]
-    lib.gk_shared_prefix_list_build.argtypes = [c_void_p] * 4 + [c_i32, c_void_p] + [c_i32] * 5 + [
+    lib.gk_shared_prefix_list_build.argtypes = [c_void_p] * 5 + [c_i32, c_void_p] + [c_i32] * 5 + [
         c_void_p, c_i64, ctypes.POINTER(SharedPrefixList)]
     lib.gk_shared_prefix_workspace_bytes.restype = ctypes.c_size_t
     lib.gk_shared_prefix_workspace_bytes.argtypes = [ctypes.POINTER(PrefillParams), ctypes.POINTER(SharedPrefixList)]

@@ -101,12 +101,12 @@ struct SharedArgs : PrefillArgs {
   uint16_t* pool_out;
 };
 
-template <int D>
+template <int D, int KEYS = prefill_keys<D>()>
 struct PrefillShape {
   static constexpr int NC = D / 32;                 // 32-dim k chunks of Q.K
   static constexpr int CPR = D / 8;                 // 16-byte chunks per head row
   static constexpr int NO = D / 16;                 // 16-dim output chunks
-  static constexpr int TILE = prefill_keys<D>() * D * 2;  // bytes of one K or V tile
+  static constexpr int TILE = KEYS * D * 2;  // bytes of one K or V tile
   static constexpr int NI = TILE / 1024;            // 1 KiB load instructions per tile
 };
 
@@ -138,8 +138,9 @@ constexpr int shared_worker_lds(int head_dim) {
 // Args: PrefillArgs, or SharedArgs for the tiles of a shared-prefix launch.
 template <int D, int SCORE, int MODE, class Args>
 __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) {
-  using S = PrefillShape<D>;
   constexpr bool SHARED = std::is_same_v<Args, SharedArgs>;
+  constexpr int kKeys = SHARED ? shared_step_keys(D) : prefill_keys<D>();
+  using S = PrefillShape<D, kKeys>;
   // Room between a base and the maximum that set it. A causal tile takes it above the base (a re-base when a score
   // exceeds the base by it: probabilities of up to 2^8), a shared one below (the base lies that far above the
   // maximum: up to 1), so that its unnormalised sums overflow only where the values' own sum does. Powers of two: the
@@ -150,7 +151,6 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
   constexpr bool LOG2 = score_capped(SCORE);  // scores in log2 units before the maxima, not raw products
   // This head dimension's query tiles per wave (in place of the namespace's).
   constexpr int kNT = prefill_nt<D>(), kQrowsPerWave = 16 * kNT;
-  constexpr int kKeys = prefill_keys<D>();
   static_assert(kKeys == 32 || kKeys == 64, "a step is one or two 32-key halves");
   constexpr int kKG = kKeys / 16;  // 16-key groups per step (Q.K tiles)
   constexpr int kKH = kKeys / 32;  // 32-key halves per step (P.V k chunks)
@@ -200,7 +200,8 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
   const int g = a.group;
   const auto div_group = [&](int x) { return (int)fast_div((uint32_t)x, a.group_div); };
   int kvh, request, first_row, nr, pos_lo, key_begin, kb0, nsteps, slot = -1;
-  [[maybe_unused]] int key_lo = 0, key_hi = 0;  // shared tiles: the keys that their rows share
+  // Shared tiles: the keys that their rows share; the batch row and position of the first row (SharedTile).
+  [[maybe_unused]] int key_lo = 0, key_hi = 0, batch_row0 = 0, pos0 = 0;
   if constexpr (SHARED) {
     asm volatile("" ::"s"(a.items), "s"(a.row_request), "s"(a.item_count), "s"(a.class_shift), "s"(a.class_heads),
                  "s"(a.class_xcds), "s"(a.class_heads_div.mul), "s"(a.class_heads_div.shift), "s"(a.block_tables),
@@ -226,7 +227,10 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
     kb0 = scalar_load(rec, 4);
     nsteps = scalar_load(rec, 5);
     slot = scalar_load(rec, 6);
-    request = scalar_load(a.row_request, scalar_load(rec, 7));
+    batch_row0 = scalar_load(rec, 7);
+    pos0 = scalar_load(rec, 8);
+    request = scalar_load(rec, 9);
+    if (request < 0) request = scalar_load(a.row_request, batch_row0);
     key_begin = max(key_lo, kb0);
     pos_lo = 0;
   } else if (a.items) {
@@ -305,48 +309,56 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
   bool qvalid[kNT];
   bf16x8_t qb[kNT][S::NC];
   [[maybe_unused]] float slope[kNT];
-#pragma unroll
-  for (int nt = 0; nt < kNT; ++nt) {
-    const int qr = wave * kQrowsPerWave + nt * 16 + c16;
-    const int row = div_group(qr), head = qr - row * g;
-    qvalid[nt] = row < nr;
-    int batch_row = first_row + row;
-    if constexpr (SHARED) {
-      // The rows share the keys [key_lo, key_hi) of the tile; their positions (and windows) are their own.
-      const int at = first_row + min(row, nr - 1);
-      batch_row = a.row_map[at];
-      const int pos = a.row_position[at];
-      qpos[nt] = qvalid[nt] ? min(pos, key_hi - 1) : -1;
-      qleft[nt] = a.window > 0 ? max(key_lo, pos - a.window + 1) : key_lo;
-    } else {
-      qpos[nt] = qvalid[nt] ? pos_lo + row : -1;
-      qleft[nt] = a.window > 0 ? qpos[nt] - a.window + 1 : 0;
-    }
-    const uint16_t* src = a.query + (int64_t)batch_row * a.q_stride + (int64_t)(kvh * g + head) * D;
-    if constexpr (score_biased(SCORE))
-      slope[nt] = qvalid[nt] ? fminf(a.slopes[kvh * g + head], kMostSlope) * (LOG2 ? kLog2e : kLog2e / a.score_scale) : 0.f;
-#pragma unroll
-    for (int c = 0; c < S::NC; ++c) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (qvalid[nt]) v = load16(src + (4 * c + q) * 8);
-      qb[nt][c] = __builtin_bit_cast(bf16x8_t, v);
-    }
-  }
-
   // Smallest query position and largest window start over this wave's valid rows.
   int wave_pos_min = pos_lo + div_group(wave * kQrowsPerWave);
   int wave_left_max =
       a.window > 0 ? pos_lo + min(nr - 1, div_group(wave * kQrowsPerWave + kQrowsPerWave - 1)) - a.window + 1 : 0;
-  if constexpr (SHARED) {
-    int low = INT32_MAX, left = 0;
+  auto load_queries = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
-      low = min(low, qvalid[nt] ? qpos[nt] : INT32_MAX);
-      left = max(left, qvalid[nt] ? qleft[nt] : 0);
+      const int qr = wave * kQrowsPerWave + nt * 16 + c16;
+      const int row = div_group(qr), head = qr - row * g;
+      qvalid[nt] = row < nr;
+      int batch_row = first_row + row;
+      if constexpr (SHARED) {
+        // The rows share the keys [key_lo, key_hi) of the tile; their positions (and windows) are their own.
+        const int at = min(row, nr - 1);
+        int pos = pos0 + at;
+        batch_row = batch_row0 + at;
+        if (pos0 < 0) {
+          batch_row = a.row_map[first_row + at];
+          pos = a.row_position[first_row + at];
+        }
+        qpos[nt] = qvalid[nt] ? min(pos, key_hi - 1) : -1;
+        qleft[nt] = a.window > 0 ? max(key_lo, pos - a.window + 1) : key_lo;
+      } else {
+        qpos[nt] = qvalid[nt] ? pos_lo + row : -1;
+        qleft[nt] = a.window > 0 ? qpos[nt] - a.window + 1 : 0;
+      }
+      const uint16_t* src = a.query + (int64_t)batch_row * a.q_stride + (int64_t)(kvh * g + head) * D;
+      if constexpr (score_biased(SCORE))
+        slope[nt] = qvalid[nt] ? fminf(a.slopes[kvh * g + head], kMostSlope) * (LOG2 ? kLog2e : kLog2e / a.score_scale) : 0.f;
+#pragma unroll
+      for (int c = 0; c < S::NC; ++c) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (qvalid[nt]) v = load16(src + (4 * c + q) * 8);
+        qb[nt][c] = __builtin_bit_cast(bf16x8_t, v);
+      }
     }
-    wave_pos_min = columns_min(low);
-    wave_left_max = -columns_min(-left);
-  }
+
+    if constexpr (SHARED) {
+      int low = INT32_MAX, left = 0;
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
+        low = min(low, qvalid[nt] ? qpos[nt] : INT32_MAX);
+        left = max(left, qvalid[nt] ? qleft[nt] : 0);
+      }
+      wave_pos_min = columns_min(low);
+      wave_left_max = -columns_min(-left);
+    }
+  };
+  // (A shared tile's come behind its first K and V tiles: a chain of round trips less before those.)
+  if constexpr (!SHARED) load_queries();
 
   // At d 128 the row sums of the bf16 probabilities run on one more MFMA per
   // half step against an all-ones operand, in the output layout (rows 4q + r).
@@ -358,7 +370,10 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
   // softmax phases (C4 shapes: 113.7 -> 104.8 us); at d 128 the same order
   // measured 158.9 -> 181.0 us, with or without the phase offset, so d 128
   // keeps one barrier per step with every wave in Q.K -> softmax -> P.V order.
-  constexpr bool kPingPong = D < 128;
+  // (A shared tile has its CU to itself and few steps: there a step of 64 keys
+  // and one barrier, whose loads have a whole step to arrive, serve head_dim 64
+  // too.)
+  constexpr bool kPingPong = D < 128 && !SHARED;
   f32x4_t o[kNT][S::NO];
   float m_run[kNT];
   // Without softcap the re-base check compares the raw score maximum with
@@ -387,7 +402,7 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
   // words made uniform with readfirstlane (the compiler keeps the opaque
   // resource in VGPRs there); d 64 keeps the builtin resource (1.8% faster).
   auto make_rsrc = [&](const uint16_t* base) {
-    if constexpr (D < 128) return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, region, kBufferDword3);
+    if constexpr (D < 128 && !SHARED) return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, region, kBufferDword3);
     else return buffer_words(base, region);
   };
   using Rsrc = decltype(make_rsrc(kbase));
@@ -460,7 +475,7 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
     for (int k = 0; k < LPW; ++k) {
       const int ins = wave + k * kPrefillWaves;
       if (S::NI % kPrefillWaves != 0 && ins >= S::NI) break;  // wave-uniform
-      if constexpr (D < 128) lds_dma16(base + ins * 1024, rs, of.v[k]);
+      if constexpr (D < 128 && !SHARED) lds_dma16(base + ins * 1024, rs, of.v[k]);
       else lds_dma16_w(base + ins * 1024, rs, of.v[k]);
     }
   };
@@ -684,6 +699,7 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
       }
       return;
     }
+    if constexpr (SHARED) load_queries();
     // The loop is unrolled over the two stages, so that every LDS address of a
     // step is a per-lane offset plus an immediate (stage, 16-key group, half):
     // ~44 fewer VALU instructions per wave and step (C4: 148.6 -> 138.0 us).

@@ -117,9 +117,9 @@ void launch_mode(const SharedArgs& a, bool softcap, dim3 grid, hipStream_t strea
 
 template <int D>
 void launch(const SharedArgs& a, bool softcap, int block_size, dim3 grid, hipStream_t stream) {
-  constexpr int keys = prefill_keys<D>();
+  constexpr int keys = shared_step_keys(D);
   if (block_size >= keys) launch_mode<D, kStepBlocks>(a, softcap, grid, stream);
-  else if (block_size >= keys / PrefillShape<D>::NI) launch_mode<D, kLoadBlocks>(a, softcap, grid, stream);
+  else if (block_size >= keys / PrefillShape<D, keys>::NI) launch_mode<D, kLoadBlocks>(a, softcap, grid, stream);
   else launch_mode<D, kKeyBlocks>(a, softcap, grid, stream);
 }
 
@@ -133,7 +133,7 @@ size_t workspace_bytes_of(const gk_prefill_params* p, const gk_shared_prefix_lis
 }  // namespace
 
 int shared_prefix_list_build(const int32_t* run_first_row, const int32_t* run_rows, const int32_t* run_pos,
-                             const int32_t* run_group, int32_t runs, const int32_t* group_prefix, int32_t groups,
+                             const int32_t* run_group, const int32_t* run_request, int32_t runs, const int32_t* group_prefix, int32_t groups,
                              int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t sliding_window,
                              int32_t* words, int64_t capacity, gk_shared_prefix_list* list) {
   const char* const name = "gk_shared_prefix_list_build";
@@ -153,12 +153,14 @@ int shared_prefix_list_build(const int32_t* run_first_row, const int32_t* run_ro
     if (run_rows[i] <= 0 || run_first_row[i] < 0 || group_prefix[g] < 0 || run_pos[i] < group_prefix[g] ||
         (int64_t)run_pos[i] + run_rows[i] > INT32_MAX - 64)
       return bad("a run's rows must lie behind its group's prefix");
+    if (run_request && run_request[i] < 0) return bad("negative request");
     rows += run_rows[i];
   }
   if (rows > 65535) return bad("too many rows");
   try {
     std::vector<SharedRun> in(runs);
-    for (int32_t i = 0; i < runs; ++i) in[i] = {run_first_row[i], run_rows[i], run_pos[i], run_group[i]};
+    for (int32_t i = 0; i < runs; ++i) 
+      in[i] = {run_first_row[i], run_rows[i], run_pos[i], run_group[i], run_request ? run_request[i] : -1};
     const SharedPlan plan =
         shared_plan(in.data(), runs, group_prefix, q_heads / kv_heads, kv_heads, head_dim, sliding_window, device_cus());
     if (plan.cols > INT32_MAX) return bad("too many partial results");
@@ -280,12 +282,13 @@ int shared_prefix_attention(const gk_prefill_params* p, const gk_shared_prefix_l
 }  // namespace gk
 
 extern "C" int gk_shared_prefix_list_build(const int32_t* run_first_row, const int32_t* run_rows,
-                                           const int32_t* run_pos, const int32_t* run_group, int32_t runs,
+                                           const int32_t* run_pos, const int32_t* run_group,
+                                           const int32_t* run_request, int32_t runs,
                                            const int32_t* group_prefix, int32_t groups, int32_t q_heads,
                                            int32_t kv_heads, int32_t head_dim, int32_t sliding_window, int32_t* words,
                                            int64_t capacity, gk_shared_prefix_list* list) {
   gk::clear_error();
-  return gk::shared_prefix_list_build(run_first_row, run_rows, run_pos, run_group, runs, group_prefix, groups, q_heads,
+  return gk::shared_prefix_list_build(run_first_row, run_rows, run_pos, run_group, run_request, runs, group_prefix, groups, q_heads,
                                       kv_heads, head_dim, sliding_window, words, capacity, list);
 }
 

@@ -24,27 +24,28 @@ namespace gk {
 // A worker is one wave: at most shared_columns columns (two 16-column tiles; one
 // at head_dim 256, where two spill 77 registers), tiles of shared_tile_keys keys.
 constexpr int shared_columns(int head_dim) { return head_dim > 128 ? 16 : 32; }
+constexpr int shared_step_keys(int head_dim) { return head_dim > 128 ? 32 : 64; }  // of a workgroup's tile
 constexpr int shared_tile_keys(int head_dim) { return head_dim > 128 ? 16 : 32; }
 constexpr int kSharedWaves = 8;  // workers of a workgroup
 
 struct SharedRun {
-  int32_t first_row, rows, pos, group;
+  int32_t first_row, rows, pos, group, request;  // request: its block-table row; -1: only the device knows
 };
 
 // A tile of a workgroup: compact rows first .. first + rows - 1, keys
-// [key_lo, key_hi) in `steps` steps of prefill_step_keys from key0 on.
+// [key_lo, key_hi) in `steps` steps of shared_step_keys from key0 on. pos >= 0:
+// the rows are the batch rows from batch_row on, at positions pos, pos + 1, ...
+// (behind all of the tile's keys, whatever they are, where no row's window starts
+// among them); else rows and positions are looked up.
 struct SharedTile {
-  int32_t first, rows, key_lo, key_hi, key0, steps, col, batch_row;
+  int32_t first, rows, key_lo, key_hi, key0, steps, col, batch_row, pos, request, pad[2];
 };
-constexpr int kSharedTileWords = 8;
+constexpr int kSharedTileWords = 12;
 // A stretch of one worker's keys: `cols` columns of the compact rows from `first`
-// on, key tiles tile0 .. tile0 + tiles - 1. pos >= 0: the rows are the batch rows
-// from batch_row on, at positions pos, pos + 1, ... (behind all of the segment's
-// keys, whatever they are, where no row's window starts among them); else they are
-// looked up. From key new_pos on, keys are the run's new tokens: those of the batch
+// on, key tiles tile0 .. tile0 + tiles - 1; rows and positions as a tile's. From key new_pos on, keys are the run's new tokens: those of the batch
 // rows from new_row on (INT32_MAX: none).
 struct SharedSegment {
-  int32_t first, cols, tile0, tiles, key_lo, key_hi, col, batch_row, pos, new_pos, new_row, pad;
+  int32_t first, cols, tile0, tiles, key_lo, key_hi, col, batch_row, pos, new_pos, new_row, request;
 };
 constexpr int kSharedSegmentWords = 12;
 // A worker's first segment, and where its others stand among the segments.
@@ -85,7 +86,7 @@ struct SharedCost {
   double bytes;       // of a worker's key tile
 };
 inline SharedCost shared_cost(int head_dim) {
-  if (head_dim == 64) return {0.65, 5.0, 1.8, 32 * 64 * 4.0};
+  if (head_dim == 64) return {1.2, 5.0, 1.8, 32 * 64 * 4.0};
   if (head_dim == 128) return {1.95, 6.0, 2.35, 32 * 128 * 4.0};
   return {1.8, 6.0, 2.35, 16 * 256 * 4.0};
 }
@@ -104,9 +105,10 @@ inline SharedPlan shared_plan(const SharedRun* runs, int count, const int32_t* g
                               int head_dim, int window, int cus) {
   SharedPlan plan;
   const int tile_cols = prefill_tile_qrows(head_dim), tile_rows = tile_cols / group;
-  const int step_keys = prefill_step_keys(head_dim), key_tile = shared_tile_keys(head_dim);
+  const int step_keys = shared_step_keys(head_dim), key_tile = shared_tile_keys(head_dim);
   const int columns = shared_columns(head_dim);
   std::vector<SharedWork> wide, narrow;
+  std::vector<int32_t> row_request;  // of compact rows
   const auto add = [&](int first, int rows, int lo, int hi, int run) {
     // Heads beyond a worker's columns go to a workgroup's tile; so do more than two workers' columns.
     if (lo >= hi) return;
@@ -139,6 +141,7 @@ inline SharedPlan shared_plan(const SharedRun* runs, int count, const int32_t* g
       for (int r = 0; r < run.rows; ++r) {
         plan.row_map.push_back(run.first_row + r);
         plan.row_position.push_back(run.pos + r);
+        row_request.push_back(run.request);
         plan.merges.push_back({0, 0, 0, 0, 0, 0, run.first_row + r, 0});
       }
       for (int r = 0; r < run.rows; r += tile_rows) {
@@ -209,6 +212,17 @@ inline SharedPlan shared_plan(const SharedRun* runs, int count, const int32_t* g
   if (narrow.empty()) workers = 0;
   const int tile_slots = std::max(1, slots - (workers + kSharedWaves - 1) / kSharedWaves);
 
+  // A record's pos (SharedTile).
+  const auto position = [&](const SharedWork& w) {
+    const int row0 = plan.row_map[w.first], pos0 = plan.row_position[w.first];
+    bool rows_follow = true, positions_follow = true;
+    for (int r = 1; r < w.rows; ++r) {
+      rows_follow = rows_follow && plan.row_map[w.first + r] == row0 + r;
+      positions_follow = positions_follow && plan.row_position[w.first + r] == pos0 + r;
+    }
+    const bool see_all = window <= 0 && w.run < 0;
+    return !rows_follow ? -1 : positions_follow ? pos0 : see_all ? w.key_hi : -1;
+  };
   const auto place = [&](const SharedWork& w, int parts) {
     // Columns of the work's parts, a multiple of 16 each.
     const int stride = (w.rows * group + 15) / 16 * 16;
@@ -226,13 +240,13 @@ inline SharedPlan shared_plan(const SharedRun* runs, int count, const int32_t* g
   if (!wide.empty()) {
     const int most = tile_pieces(tile_slots);
     for (const auto& w : wide) {
-      const int parts = (w.units + most - 1) / most;
+      const int parts = (w.units + most - 1) / most, pos = position(w);
       const int64_t col = place(w, parts);
       const int stride = (w.rows * group + 15) / 16 * 16;
       for (int p = 0, done = 0; p < parts; ++p) {
         const int end = (int)(int64_t{w.units} * (p + 1) / parts);
         plan.tiles.push_back({w.first, w.rows, w.key_lo, w.key_hi, w.start + done * step_keys, end - done,
-                              (int32_t)(col + int64_t{p} * stride), plan.row_map[w.first]});
+                              (int32_t)(col + int64_t{p} * stride), plan.row_map[w.first], pos, row_request[w.first], {0, 0}});
         done = end;
       }
     }
@@ -274,21 +288,14 @@ inline SharedPlan shared_plan(const SharedRun* runs, int count, const int32_t* g
     size_t at = 0, worker = 0;
     for (size_t i = 0; i < narrow.size(); ++i) {
       const SharedWork& w = narrow[i];
-      const int row0 = plan.row_map[w.first], pos0 = plan.row_position[w.first];
-      bool rows_follow = true, positions_follow = true;
-      for (int r = 1; r < w.rows; ++r) {
-        rows_follow = rows_follow && plan.row_map[w.first + r] == row0 + r;
-        positions_follow = positions_follow && plan.row_position[w.first + r] == pos0 + r;
-      }
-      const bool see_all = window <= 0 && w.run < 0;
-      const int pos = !rows_follow ? -1 : positions_follow ? pos0 : see_all ? w.key_hi : -1;
+      const int pos = position(w);
       const int64_t col = place(w, pieces_of[i]);
       const int stride = (w.rows * group + 15) / 16 * 16;
       for (int p = 0, done = 0; p < pieces_of[i]; ++p, ++at) {
         const SharedSegment seg{w.first, w.rows * group, w.start / key_tile + done, piece_ends[at] - done, w.key_lo,
                                 w.key_hi, (int32_t)(col + int64_t{p} * stride), plan.row_map[w.first], pos,
                                 w.run < 0 ? INT32_MAX : plan.row_position[w.run],
-                                w.run < 0 ? 0 : plan.row_map[w.run], 0};
+                                w.run < 0 ? 0 : plan.row_map[w.run], row_request[w.first]};
         done = piece_ends[at];
         if ((int32_t)at == worker_segs[worker]) {
           plan.workers.push_back({seg, (int32_t)plan.segs.size(), (int32_t)plan.segs.size(), {0, 0}});

@@ -45,12 +45,12 @@ __device__ __forceinline__ void lds_dma4_w(uint32_t lds, u32x4_t rsrc, uint32_t 
 
 // A segment's record (SharedSegment) in scalar registers.
 struct SegmentWords {
-  int first, ncols, tile0, ntiles, key_lo, key_hi, col, batch_row, pos, new_pos, new_row;
+  int first, ncols, tile0, ntiles, key_lo, key_hi, col, batch_row, pos, new_pos, new_row, request;
 };
 __device__ __forceinline__ SegmentWords load_segment(const int32_t* rec) {
   return {scalar_load(rec, 0), scalar_load(rec, 1), scalar_load(rec, 2), scalar_load(rec, 3), scalar_load(rec, 4),
           scalar_load(rec, 5), scalar_load(rec, 6), scalar_load(rec, 7), scalar_load(rec, 8), scalar_load(rec, 9),
-          scalar_load(rec, 10)};
+          scalar_load(rec, 10), scalar_load(rec, 11)};
 }
 
 // NT: 16-column tiles of the segment. `meanwhile` runs once its first loads are on their way.
@@ -351,12 +351,16 @@ __device__ __forceinline__ void shared_worker(const SharedArgs& a, char* lds, in
   // The next segment's record, and the request behind it, come while a segment runs.
   const int32_t* rec = a.worker_list + (int64_t)worker * kSharedWorkerWords;
   SegmentWords seg = load_segment(rec), next;
-  int at = scalar_load(rec, kSharedSegmentWords), request = scalar_load(a.row_request, seg.batch_row), next_request = 0;
+  int at = scalar_load(rec, kSharedSegmentWords), next_request = 0;
+  const auto request_of = [&](const SegmentWords& s) {
+    return s.request >= 0 ? s.request : scalar_load(a.row_request, s.batch_row);
+  };
+  int request = request_of(seg);
   const int end = scalar_load(rec, kSharedSegmentWords + 1);
   for (;;) {
     const bool more = at < end;
     next = more ? load_segment(a.segs + (int64_t)at * kSharedSegmentWords) : seg;
-    const auto meanwhile = [&] { next_request = scalar_load(a.row_request, next.batch_row); };
+    const auto meanwhile = [&] { next_request = request_of(next); };
     const int32_t* bt = a.block_tables + (int64_t)request * a.bt_stride;
     if (shared_columns(D) == 16 || seg.ncols <= 16)
       shared_segment<D, SCORE, 1>(a, kt, entries, kvh, seg, bt, meanwhile);

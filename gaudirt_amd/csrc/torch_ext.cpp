@@ -890,7 +890,7 @@ class PagedMetadata : public torch::CustomClassHolder {
     // Runs, cut where groups meet. A run that fills a tile of the prefill kernel
     // reads its keys once for all of the tile's columns already: it gains nothing
     // from its group.
-    std::vector<int32_t> first, rows, pos, of_group, prefix(group_prefix.begin(), group_prefix.end());
+    std::vector<int32_t> first, rows, pos, of_group, request, prefix(group_prefix.begin(), group_prefix.end());
     std::vector<int32_t> chunk_first, chunk_rows, chunk_pos;
     int64_t g = 0, group_end = group_rows[0];
     // A host request map says which rows are one request's. Where each request is
@@ -908,6 +908,7 @@ class PagedMetadata : public torch::CustomClassHolder {
         (chunk ? chunk_rows : rows).push_back(static_cast<int32_t>(end - r));
         (chunk ? chunk_pos : pos).push_back(static_cast<int32_t>(run.prefix + (r - run.row)));
         if (!chunk) of_group.push_back(static_cast<int32_t>(g));
+        if (!chunk && !mapping_h_.empty()) request.push_back(requests_h_[run.row]);
         r = end;
       }
     }
@@ -924,7 +925,8 @@ class PagedMetadata : public torch::CustomClassHolder {
       work.resize(64 * rows.size() + 8192);
       for (;;) {
         const int rc = gk_shared_prefix_list_build(
-            first.data(), rows.data(), pos.data(), of_group.data(), static_cast<int32_t>(rows.size()), prefix.data(),
+            first.data(), rows.data(), pos.data(), of_group.data(), request.empty() ? nullptr : request.data(),
+            static_cast<int32_t>(rows.size()), prefix.data(),
             static_cast<int32_t>(prefix.size()), static_cast<int32_t>(query_heads), static_cast<int32_t>(kv_heads),
             static_cast<int32_t>(head_dim), static_cast<int32_t>(window), work.data(),
             static_cast<int64_t>(work.size()), &plan.shared);

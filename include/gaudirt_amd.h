@@ -252,7 +252,8 @@ int gk_paged_prefill_alibi(const gk_prefill_params* params, const gk_prefill_lis
  *
  * gk_shared_prefix_list_build (host only) plans the work of host-known lengths:
  * it fills `list` but for its two pointers and writes word_count words
- * (GK_ERR_WORKSPACE, with word_count set, when capacity is smaller). The caller
+ * (GK_ERR_WORKSPACE, with word_count set, when capacity is smaller). run_request:
+ * block-table row of each run, or NULL where only the device knows them. The caller
  * copies the words to the device, 16-byte aligned, and sets words to the copy
  * and row_request to the block-table row of every batch row (device). The new
  * tokens are in the pool before the call or, where the list says can_store and
@@ -276,7 +277,7 @@ typedef struct gk_shared_prefix_list {
 } gk_shared_prefix_list;
 
 int gk_shared_prefix_list_build(const int32_t* run_first_row, const int32_t* run_rows, const int32_t* run_pos,
-                                const int32_t* run_group, int32_t runs, const int32_t* group_prefix, int32_t groups,
+                                const int32_t* run_group, const int32_t* run_request, int32_t runs, const int32_t* group_prefix, int32_t groups,
                                 int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t sliding_window,
                                 int32_t* words, int64_t capacity, gk_shared_prefix_list* list);
 size_t gk_shared_prefix_workspace_bytes(const gk_prefill_params* params, const gk_shared_prefix_list* list);

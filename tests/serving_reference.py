@@ -149,7 +149,7 @@ def same_bits(a, b):
     return torch.equal(a.view(torch.int16), b.view(torch.int16))
 
 
-def shared_prefix_c(b, softcap=0.0, window=-1, ride_along=False, page=None):
+def shared_prefix_c(b, softcap=0.0, window=-1, ride_along=False, known_requests=True, page=None):
     """The batch through gk_shared_prefix_list_build and gk_shared_prefix_attention, whatever its size (the operator
     lets short batches attend row by row): the new rows stored by gk_kv_store first, or with ride_along by the call
     itself. Rows of the output that the call does not write are NaN."""
@@ -159,9 +159,11 @@ def shared_prefix_c(b, softcap=0.0, window=-1, ride_along=False, page=None):
     first = as_i32(np.concatenate([[0], np.cumsum(news)[:-1]]))
     pos = as_i32([b.prefix[g] + own for g, own, _ in b.requests])
     group, prefix = as_i32([g for g, _, _ in b.requests]), as_i32(b.group_prefix)
+    request = as_i32(np.arange(len(news)))
     host = lambda a: ctypes.c_void_p(a.ctypes.data)  # noqa: E731
     words, lst = np.zeros(1 << 20, dtype=np.int32), capi.SharedPrefixList()
-    capi.check(lib.gk_shared_prefix_list_build(host(first), host(news), host(pos), host(group), len(news), host(prefix),
+    capi.check(lib.gk_shared_prefix_list_build(host(first), host(news), host(pos), host(group), host(request) if known_requests else None,
+                                               len(news), host(prefix),
                                                len(prefix), b.q_heads, b.kv_heads, b.d, window, host(words), words.size,
                                                ctypes.byref(lst)))
     device_words = torch.from_numpy(words[:lst.word_count].copy()).cuda()

@@ -26,7 +26,7 @@ void check(const std::vector<gk::SharedRun>& runs, const std::vector<int32_t>& p
   const auto plan = gk::shared_plan(runs.data(), (int)runs.size(), prefix.data(), group, kv_heads, d, window, 256);
   std::vector<gk::SharedRun> row_run;
   for (const auto& run : runs)
-    for (int r = 0; r < run.rows; ++r) row_run.push_back({run.first_row + r, 1, run.pos + r, run.group});
+    for (int r = 0; r < run.rows; ++r) row_run.push_back({run.first_row + r, 1, run.pos + r, run.group, run.request});
   const size_t rows = row_run.size();
   expect(plan.row_map.size() == rows && plan.row_position.size() == rows && plan.merges.size() == rows, "row count", trial);
   for (size_t i = 0; i < rows; ++i)
@@ -47,11 +47,17 @@ void check(const std::vector<gk::SharedRun>& runs, const std::vector<int32_t>& p
     }
     pieces[col] = {first, n, lo, hi};
   };
-  const int step = gk::prefill_step_keys(d), tile = gk::shared_tile_keys(d);
+  const int step = gk::shared_step_keys(d), tile = gk::shared_tile_keys(d);
   for (size_t i = 0; i < plan.tiles.size(); ++i) {
     const auto& t = plan.tiles[i];
     expect(t.steps > 0 && t.key0 % step == 0, "a tile's steps", trial);
     expect(t.rows * group <= gk::prefill_tile_qrows(d), "a tile's columns", trial);
+    expect(t.request == row_run[t.first].request, "a tile's request", trial);
+    for (int r = 0; t.pos >= 0 && r < t.rows; ++r)
+      expect(plan.row_map[t.first + r] == t.batch_row + r &&
+                 (t.pos + r == row_run[t.first + r].pos ||
+                  (window <= 0 && std::min(t.pos + r, row_run[t.first + r].pos) >= t.key_hi - 1)),
+             "a tile's rows and positions", trial);
     expect(i == 0 || plan.tiles[i - 1].steps >= t.steps, "tiles are not longest first", trial);
     add(t.first, t.rows, std::max(t.key_lo, t.key0), std::min(t.key_hi, t.key0 + t.steps * step), t.col, t.batch_row);
   }
@@ -59,6 +65,7 @@ void check(const std::vector<gk::SharedRun>& runs, const std::vector<int32_t>& p
     expect(s.tiles > 0 && s.cols > 0 && s.cols <= gk::shared_columns(d) && s.cols % group == 0, "a segment", trial);
     add(s.first, s.cols / group, std::max(s.key_lo, s.tile0 * tile), std::min(s.key_hi, (s.tile0 + s.tiles) * tile), s.col,
         s.batch_row);
+    expect(s.request == row_run[s.first].request, "a segment's request", trial);
     // New tokens: the run's rows, seen by a run's own segments only.
     if (s.new_pos != INT32_MAX) {
       const gk::SharedRun* run = nullptr;
@@ -141,7 +148,7 @@ int main() {
       const int count = pick(1, trial % 5 ? 5 : 60);
       for (int i = 0; i < count; ++i) {
         const int n = pick(0, 2) ? 1 : pick(1, trial % 7 ? 8 : 150);
-        runs.push_back({row, n, prefix[k] + (pick(0, 2) ? pick(0, 900) : 0), k});
+        runs.push_back({row, n, prefix[k] + (pick(0, 2) ? pick(0, 900) : 0), k, trial % 2 ? (int)runs.size() : -1});
         row += n + (pick(0, 9) == 0);
       }
     }

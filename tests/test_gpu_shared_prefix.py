@@ -35,6 +35,7 @@ def check(b, **kind):
         stored, can_store = shared_prefix_c(b, **kind)
         b.check(stored, **kind)
         assert same_bits(b.pool, expected_pool)
+        assert same_bits(shared_prefix_c(b, known_requests=False, **kind)[0], stored)
         if can_store:
             b.pool.copy_(before)
             along, _ = shared_prefix_c(b, ride_along=True, **kind)

@@ -25,7 +25,7 @@ def test_plan_covers_every_key_once(tmp_path):
 
 
 def build(first=(0, 1), rows=(1, 1), pos=(700, 900), group=(0, 0), prefix=(640,), heads=(32, 8, 128), window=-1,
-          capacity=1 << 16, size=None):
+          capacity=1 << 16, size=None, request=None):
     lib, as_i32 = capi.load(), lambda a: np.ascontiguousarray(a, dtype=np.int32)
     arrays = [as_i32(a) for a in (first, rows, pos, group)]
     prefix = as_i32(prefix)
@@ -33,7 +33,8 @@ def build(first=(0, 1), rows=(1, 1), pos=(700, 900), group=(0, 0), prefix=(640,)
     if size is not None:
         lst.struct_size = size
     ptr = lambda a: ctypes.c_void_p(a.ctypes.data)  # noqa: E731
-    rc = lib.gk_shared_prefix_list_build(*map(ptr, arrays), len(arrays[0]), ptr(prefix), len(prefix), *heads, window,
+    request = None if request is None else as_i32(request)
+    rc = lib.gk_shared_prefix_list_build(*map(ptr, arrays), None if request is None else ptr(request), len(arrays[0]), ptr(prefix), len(prefix), *heads, window,
                                          ptr(words), capacity, ctypes.byref(lst))
     return rc, words, lst
 
@@ -59,7 +60,7 @@ def test_list_has_its_words():
     ({"pos": (639, 900)}, "behind its group's prefix"), ({"rows": (0, 1)}, "behind its group's prefix"),
     ({"prefix": (-1,)}, "behind its group's prefix"), ({"pos": (700, 2**31 - 40)}, "behind its group's prefix"),
     ({"rows": (65000, 1000)}, "too many rows"), ({"first": (), "rows": (), "pos": (), "group": ()}, "runs or groups"),
-    ({"prefix": ()}, "runs or groups"),
+    ({"prefix": ()}, "runs or groups"), ({"request": (0, -1)}, "negative request"),
 ])
 def test_build_refuses(change, message):
     rc, words, _ = build(**change)
