@@ -12,9 +12,10 @@
 // One launch. Every workgroup makes the three sums for itself, in LDS (8 bytes a
 // sequence from L2 and one scan: 1.5 us for 1024 sequences), so nothing waits
 // for another workgroup; then all threads share the rows, pages and copied
-// tokens, four in a row each, whose sequence a binary search finds. What bounds
-// it is the launch and that chain of round trips for a decode step, writing the
-// map for long prompts.
+// tokens, whose sequence a binary search finds. What bounds a decode step is the
+// launch and that chain of round trips; the code is kept small for it (rows four
+// at a time, with 64-bit indexes, were slower: most of such a call is the code's
+// own way into the instruction caches).
 #include "gk_common.hpp"
 
 #include <algorithm>
@@ -23,7 +24,6 @@ namespace gk {
 namespace {
 
 constexpr int kThreads = 512, kWaves = kThreads / 64;
-constexpr int kPerThread = 4;  // consecutive rows, pages or tokens of a thread
 constexpr int kSmallBatch = 1024;
 constexpr int kMaxBatch = GK_EXTEND_MAX_BATCH;
 
@@ -48,8 +48,12 @@ struct ExtendArgs {
   int32_t* counts;
 };
 
+// Element i of an int32 or int64 vector, without a branch on the type (a load
+// whose value a branch converts is waited for there, one after the other).
 __device__ __forceinline__ int64_t load_index(const void* p, int is64, int64_t i) {
-  return is64 ? static_cast<const int64_t*>(p)[i] : (int64_t) static_cast<const int32_t*>(p)[i];
+  const int32_t* w = static_cast<const int32_t*>(p) + (i << is64);
+  const int32_t low = w[0], high = w[is64];
+  return is64 ? (int64_t)((uint64_t)(uint32_t)high << 32 | (uint32_t)low) : (int64_t)low;
 }
 
 // Sums that end at INT32_MAX instead of passing it: a batch whose sum gets there is refused.
@@ -61,27 +65,48 @@ struct Sums {
 __device__ __forceinline__ Sums operator+(const Sums& a, const Sums& b) {
   return {add_sat(a.rows, b.rows), add_sat(a.pages, b.pages), add_sat(a.copies, b.copies)};
 }
-__device__ __forceinline__ Sums shift_up(const Sums& a, int n) {
-  return {(uint32_t)__shfl_up((int)a.rows, n), (uint32_t)__shfl_up((int)a.pages, n), (uint32_t)__shfl_up((int)a.copies, n)};
+// The sum of the lanes up to this one, with DPP shifts (a source outside the row reads 0).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ Sums shifted(const Sums& a) {
+  const auto move = [](uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, ROWS == 0xf);
+  };
+  return {move(a.rows), move(a.pages), move(a.copies)};
+}
+__device__ __forceinline__ Sums wave_inclusive(Sums x) {
+  x = x + shifted<0x111, 0xf>(x);  // row_shr:1
+  x = x + shifted<0x112, 0xf>(x);  // row_shr:2
+  x = x + shifted<0x114, 0xf>(x);  // row_shr:4
+  x = x + shifted<0x118, 0xf>(x);  // row_shr:8
+  x = x + shifted<0x142, 0xa>(x);  // row_bcast:15, rows 1 and 3
+  x = x + shifted<0x143, 0xc>(x);  // row_bcast:31, rows 2 and 3
+  return x;
 }
 
-// Last s with first[s] <= x (first[0] = 0 <= x < first[n]): the sequence that owns x, empty ones passed over.
-__device__ __forceinline__ int owner(const int32_t* first, int n, int x) {
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (first[mid] <= x) lo = mid;
-    else hi = mid;
+// The last s < n with first[s] <= x (first[0] = 0 <= x < first[n]): the sequence that owns x, empty ones passed over.
+// `top`: the largest power of two below n, or 0.
+__device__ __forceinline__ int owner(const int32_t* first, int n, int top, int x) {
+  int s = 0;
+  for (int step = top; step; step >>= 1) {
+    const int mid = s + step;
+    s = mid < n && first[mid] <= x ? mid : s;
   }
-  return lo;
+  return s;
 }
 
 template <int MAX>
 __global__ __launch_bounds__(kThreads) void extend_tables_kernel(ExtendArgs a) {
+  // A sequence's table row, its parent's and the page that its first new token may continue as well, where the LDS has
+  // room for them (8192 sequences leave them in memory): known before the sums are.
+  constexpr bool kInLds = MAX <= kSmallBatch;
+  constexpr int kExtra = kInLds ? MAX : 1;
   __shared__ int32_t s_row[MAX + 1], s_page[MAX + 1], s_copy[MAX + 1], s_prefix[MAX];
+  __shared__ int32_t s_request[kExtra], s_parent[kExtra], s_last[kExtra];
   __shared__ Sums s_wave[kWaves];
   __shared__ uint32_t s_bad;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, P = 1 << a.shift;
+  // Table and map elements, tokens of a row and slots stay below 2^31 (checked on the host or below): 32-bit indexes.
+  const auto pages_of = [&](int tokens) { return (int)(((uint32_t)tokens + (uint32_t)(P - 1)) >> a.shift); };
   const int head = a.free_head ? *a.free_head : 0;
   const int copy_shift = a.mapping ? 0 : a.shift;  // copies are numbered by token with a map, else by page
   if (tid == 0) s_bad = UINT32_MAX;
@@ -89,10 +114,15 @@ __global__ __launch_bounds__(kThreads) void extend_tables_kernel(ExtendArgs a) {
 
   // A thread's sequences, their sums and the first one that cannot be right:
   // (index << 3 | code), the smallest over the batch.
-  const int per = (a.batch + kThreads - 1) / kThreads, s0 = min(a.batch, tid * per), s1 = min(a.batch, s0 + per);
+  constexpr int kPer = MAX / kThreads;  // sequences of a thread
+  const int s0 = tid * kPer;
   uint32_t bad = UINT32_MAX;
   Sums mine{0, 0, 0};
-  for (int s = s0; s < s1; ++s) {
+  [[maybe_unused]] int32_t last[kInLds ? kPer : 1];
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
+    const int s = s0 + u;
+    if (s >= a.batch) break;
     const int64_t request = load_index(a.seq_requests, a.requests64, s), prefix = load_index(a.prefixes, a.lengths64, s),
                   length = load_index(a.lengths, a.lengths64, s),
                   parent = a.parents ? load_index(a.parents, a.requests64, s) : -1;
@@ -104,33 +134,37 @@ __global__ __launch_bounds__(kThreads) void extend_tables_kernel(ExtendArgs a) {
     if (code) {
       bad = min(bad, (uint32_t)s << 3 | (uint32_t)code);
     } else {
-      const int64_t held = (prefix + P - 1) >> a.shift;
-      mine = mine + Sums{(uint32_t)length, (uint32_t)(((prefix + length + P - 1) >> a.shift) - held),
+      mine = mine + Sums{(uint32_t)length, (uint32_t)(pages_of((int)(prefix + length)) - pages_of((int)prefix)),
                          parent >= 0 ? (uint32_t)prefix >> copy_shift : 0u};
+    }
+    if constexpr (kInLds) {
+      s_request[s] = (int32_t)(code ? 0 : request);
+      s_parent[s] = (int32_t)(code ? -1 : parent);
+      last[u] = !code && (prefix & (P - 1)) ? a.tables[(int)request * a.pages + ((int)prefix >> a.shift)] : -1;
     }
     s_prefix[s] = (int32_t)(code ? 0 : prefix);
     s_row[s] = code ? 0 : (int32_t)length;  // kept for the second pass
     s_copy[s] = !code && parent >= 0;
   }
-  Sums scan = mine;
-#pragma unroll
-  for (int n = 1; n < 64; n <<= 1) {
-    const Sums below = shift_up(scan, n);
-    if (lane >= n) scan = scan + below;
-  }
+  const Sums scan = wave_inclusive(mine);
   if (lane == 63) s_wave[wave] = scan;
   __syncthreads();
-  Sums at = shift_up(scan, 1), total{0, 0, 0};
-  if (lane == 0) at = Sums{0, 0, 0};
+  Sums at{0, 0, 0}, total{0, 0, 0};
   for (int w = 0; w < kWaves; ++w) {
     if (w < wave) at = at + s_wave[w];
     total = total + s_wave[w];
   }
+  const Sums below{(uint32_t)__shfl_up((int)scan.rows, 1), (uint32_t)__shfl_up((int)scan.pages, 1),
+                   (uint32_t)__shfl_up((int)scan.copies, 1)};
+  if (lane) at = at + below;
   const int64_t free_left = head >= 0 && head <= a.free_count ? a.free_count - head : 0;
-  for (int s = s0; s < s1; ++s) {
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
+    const int s = s0 + u;
+    if (s >= a.batch) break;
     const int length = s_row[s], prefix = s_prefix[s];
-    const Sums one{(uint32_t)length,
-                   (uint32_t)((((int64_t)prefix + length + P - 1) >> a.shift) - (((int64_t)prefix + P - 1) >> a.shift)),
+    if constexpr (kInLds) s_last[s] = last[u];
+    const Sums one{(uint32_t)length, (uint32_t)(pages_of(prefix + length) - pages_of(prefix)),
                    s_copy[s] ? (uint32_t)prefix >> copy_shift : 0u};
     s_row[s] = (int32_t)at.rows;
     s_page[s] = (int32_t)at.pages;
@@ -164,65 +198,55 @@ __global__ __launch_bounds__(kThreads) void extend_tables_kernel(ExtendArgs a) {
       a.counts[3] = ok ? -1 : (int32_t)(first_bad >> 3);
     }
   }
+  const auto request_of = [&](int s) {
+    if constexpr (kInLds) return s_request[s];
+    else return (int32_t)load_index(a.seq_requests, a.requests64, s);
+  };
+  const auto parent_of = [&](int s) {
+    if constexpr (kInLds) return s_parent[s];
+    else return (int32_t)load_index(a.parents, a.requests64, s);
+  };
   // A page of the free list, -1 where it lies outside the pool.
   const auto page_at = [&](int i) {
     const int64_t page = load_index(a.free_pages, a.pages64, (int64_t)head + i);
     return page >= 0 && page < (a.slots >> a.shift) ? (int32_t)page : -1;
   };
-  const int64_t threads = (int64_t)gridDim.x * kThreads, thread = (int64_t)blockIdx.x * kThreads + tid;
+  const int threads = gridDim.x * kThreads, thread = blockIdx.x * kThreads + tid;
+  const int top = a.batch > 1 ? 1 << (31 - __builtin_clz(a.batch - 1)) : 0;
 
   // Rows: slot, request and position of every new token; rows behind the last are no tokens.
-  for (int64_t r0 = thread * kPerThread; r0 < a.max_rows; r0 += threads * kPerThread) {
-    const int n = (int)min((int64_t)kPerThread, a.max_rows - r0);
-    int s = r0 < rows ? owner(s_row, a.batch, (int)r0) : 0;
-    int last_entry = -1, last_page = -1, last_seq = -1;
-    int64_t request = 0;
-    for (int k = 0; k < n; ++k) {
-      const int r = (int)r0 + k;
-      int32_t slot = -1, position = 0, where = 0;
-      if (r < rows) {
-        while (r >= s_row[s + 1]) ++s;
-        const int prefix = s_prefix[s], held = (int)(((int64_t)prefix + P - 1) >> a.shift);
-        position = prefix + (r - s_row[s]);
-        const int entry = position >> a.shift;
-        if (s != last_seq) request = load_index(a.seq_requests, a.requests64, s);
-        if (s != last_seq || entry != last_entry)
-          last_page = entry < held ? a.tables[request * a.pages + entry] : page_at(s_page[s] + entry - held);
-        last_seq = s;
-        last_entry = entry;
-        slot = last_page >= 0 ? (int32_t)(((int64_t)last_page << a.shift) + (position & (P - 1))) : -1;
-        where = (int32_t)request;
-        if (a.mapping) a.mapping[request * a.context + position] = slot;
-      }
-      a.out_locations[r] = slot;
-      a.out_requests[r] = where;
-      a.out_positions[r] = position;
+  for (int row = thread; row < a.max_rows; row += threads) {
+    int32_t slot = -1, request = 0, position = 0;
+    if (row < rows) {
+      const int s = owner(s_row, a.batch, top, row), prefix = s_prefix[s], held = pages_of(prefix);
+      request = request_of(s);
+      position = prefix + (row - s_row[s]);
+      const int entry = position >> a.shift;
+      int32_t page;
+      if (entry >= held) page = page_at(s_page[s] + entry - held);
+      else if constexpr (kInLds) page = s_last[s];  // the one page that cached tokens share with new ones
+      else page = a.tables[request * a.pages + entry];
+      if (page >= 0) slot = (page << a.shift) + (position & (P - 1));
+      if (a.mapping) a.mapping[request * a.context + position] = slot;
     }
+    a.out_locations[row] = slot;
+    a.out_requests[row] = request;
+    a.out_positions[row] = position;
   }
-  // New pages into the tables.
-  for (int64_t p = thread; p < pages; p += threads) {
-    const int s = owner(s_page, a.batch, (int)p);
-    const int held = (int)(((int64_t)s_prefix[s] + P - 1) >> a.shift);
-    const int64_t request = load_index(a.seq_requests, a.requests64, s);
-    a.tables[request * a.pages + held + ((int)p - s_page[s])] = page_at((int)p);
+  // New pages into the tables, from the last workgroup on: the first ones have the rows.
+  for (int i = threads - 1 - thread; i < pages; i += threads) {
+    const int s = owner(s_page, a.batch, top, i);
+    a.tables[request_of(s) * a.pages + pages_of(s_prefix[s]) + (i - s_page[s])] = page_at(i);
   }
-  // The parents' tokens and pages into their children's rows.
-  for (int64_t c0 = thread * kPerThread; c0 < copies; c0 += threads * kPerThread) {
-    const int n = (int)min((int64_t)kPerThread, copies - c0);
-    int s = owner(s_copy, a.batch, (int)c0), last_seq = -1;
-    int64_t request = 0, parent = 0;
-    for (int k = 0; k < n; ++k) {
-      const int c = (int)c0 + k;
-      while (c >= s_copy[s + 1]) ++s;
-      if (s != last_seq) {
-        request = load_index(a.seq_requests, a.requests64, s);
-        parent = load_index(a.parents, a.requests64, s);
-        last_seq = s;
-      }
-      const int t = (c - s_copy[s]) << copy_shift;
-      if (a.mapping) a.mapping[request * a.context + t] = a.mapping[parent * a.context + t];
-      if (!(t & (P - 1))) a.tables[request * a.pages + (t >> a.shift)] = a.tables[parent * a.pages + (t >> a.shift)];
-    }
+  // The parents' tokens and pages into their children's rows, by the workgroups without rows where there are others.
+  const int busy = min((rows + kThreads - 1) / kThreads, (int)gridDim.x / 2);
+  if ((int)blockIdx.x < busy) return;
+  const int copiers = threads - busy * kThreads;
+  for (int64_t i = thread - busy * kThreads; i < copies; i += copiers) {
+    const int s = owner(s_copy, a.batch, top, (int)i), t = ((int)i - s_copy[s]) << copy_shift;
+    const int request = request_of(s), parent = parent_of(s);
+    if (a.mapping) a.mapping[request * a.context + t] = a.mapping[parent * a.context + t];
+    if (!(t & (P - 1))) a.tables[request * a.pages + (t >> a.shift)] = a.tables[parent * a.pages + (t >> a.shift)];
   }
 }
 
@@ -269,9 +293,9 @@ int extend_block_tables(const gk_extend_params* p, hipStream_t stream) {
   a.out_positions = p->out_positions;
   a.out_lengths = p->out_lengths;
   a.counts = p->counts;
-  // Enough threads for the rows; a map's copies, whose number the host does not know, get a whole GPU's.
-  const int64_t wanted = ((int64_t)p->max_rows + kThreads * kPerThread - 1) / (kThreads * kPerThread);
-  const unsigned grid = p->parents ? 256u : (unsigned)std::max<int64_t>(1, std::min<int64_t>(wanted, 512));
+  // A thread a row up to 512 workgroups; copies, whose number the host does not know, get a whole GPU's.
+  const int64_t wanted = ((int64_t)p->max_rows + kThreads - 1) / kThreads;
+  const unsigned grid = (unsigned)std::max<int64_t>(p->parents ? 256 : 1, std::min<int64_t>(wanted, 512));
   if (p->batch <= kSmallBatch) extend_tables_kernel<kSmallBatch><<<grid, kThreads, 0, stream>>>(a);
   else extend_tables_kernel<kMaxBatch><<<grid, kThreads, 0, stream>>>(a);
   return hip_status(hipGetLastError(), "gk_extend_block_tables launch");
