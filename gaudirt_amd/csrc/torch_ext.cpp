@@ -882,6 +882,9 @@ class PagedMetadata : public torch::CustomClassHolder {
     const auto cached = shared_plans_.find(key);
     if (cached != shared_plans_.end()) return cached->second;
     check_groups(group_rows, group_prefix);
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    TORCH_CHECK(hipStreamIsCapturing(current_stream(), &capture) == hipSuccess && capture == hipStreamCaptureStatusNone,
+                "GaudiRT shared-prefix attention: the first call for these groups uploads their plan and cannot be captured");
     SharedPrefixPlan plan;
     plan.by_itself = query_heads / kv_heads > 128 || attends_in_one_launch(query_heads, kv_heads, head_dim, window);
     if (plan.by_itself) return shared_plans_.emplace(std::move(key), std::move(plan)).first->second;
@@ -1017,12 +1020,15 @@ class PagedMetadata : public torch::CustomClassHolder {
       // The host's own copy of the request map says whether the prefix is shared;
       // a device map is the caller's word.
       if (!mapping_h_.empty()) {
+        // (Visible tokens follow each other inside a page: the pages' first ones say it all.)
         const int32_t* shared = mapping_h_.data() + static_cast<int64_t>(requests_h_[row]) * context_;
-        for (int64_t r = row + 1; r < row + group_rows[g]; ++r)
-          if (requests_h_[r] != requests_h_[r - 1])
-            TORCH_CHECK(std::memcmp(shared, mapping_h_.data() + static_cast<int64_t>(requests_h_[r]) * context_,
-                                    group_prefix[g] * sizeof(int32_t)) == 0,
-                        "GaudiRT shared-prefix attention: the rows of a group do not share its prefix");
+        for (int64_t r = row + 1; r < row + group_rows[g]; ++r) {
+          if (requests_h_[r] == requests_h_[r - 1]) continue;
+          const int32_t* own = mapping_h_.data() + static_cast<int64_t>(requests_h_[r]) * context_;
+          int32_t differ = 0;
+          for (int64_t t = 0; t < group_prefix[g]; t += page_) differ |= shared[t] ^ own[t];
+          TORCH_CHECK(!differ, "GaudiRT shared-prefix attention: the rows of a group do not share its prefix");
+        }
       }
       row += group_rows[g];
     }

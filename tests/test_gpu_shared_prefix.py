@@ -274,6 +274,37 @@ def test_captured_and_replayed():
     torch.cuda.synchronize()
 
 
+def test_first_call_is_not_captured():
+    b = Batch(32, decode(1, 20, 100), [2640])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        b.metadata = b.make_metadata()
+        torch.ops.gaudirt.paged_attn(*b.inputs(), b.d, b.scale)  # the attention plan itself is there
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            with torch.cuda.graph(graph, stream=side):
+                run(b)
+        check(b)
+    torch.cuda.synchronize()
+
+
+def test_page_aligned_prefixes_that_differ_in_one_page():
+    b = Batch(33, decode(1, 9, 60), [2560], page=128)
+    for page in (0, 7, 19):
+        mapping = b.mapping.copy()
+        other = np.setdiff1d(np.arange(b.slots // 128), mapping[mapping >= 0] // 128)[0]
+        mapping[4, page * 128:(page + 1) * 128] = other * 128 + np.arange(128)
+        metadata = torch.classes.gaudirt.PagedMetadata(
+            torch.from_numpy(b.locations), torch.from_numpy(b.row_request), torch.from_numpy(b.positions),
+            torch.from_numpy(mapping), b.slots)
+        with pytest.raises(RuntimeError, match="do not share"):
+            run(b, metadata=metadata)
+        out = run(b, metadata=metadata, group_prefix=[page * 128])  # shared up to there
+        assert torch.isfinite(out[[i for i in range(9) if i != 4]]).all()
+
+
 def test_pool_beyond_32_bit_offsets():
     # Eight heads' K of 2^20 slots are 2 GiB; the last heads' rows lie past 2^32 bytes.
     b = Batch(26, decode(1, 6, 70), [160], heads=(16, 8, 256), page=16, spare=1 << 16)
