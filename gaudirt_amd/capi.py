@@ -107,6 +107,7 @@ class SharedPrefixList(_Sized):
         ("part_cols", c_i64),
         ("rows", c_i32), ("tile_count", c_i32), ("workers", c_i32), ("worker_groups", c_i32), ("word_count", c_i32),
         ("can_store", c_i32),
+        ("q_heads", c_i32), ("kv_heads", c_i32), ("head_dim", c_i32), ("sliding_window", c_i32),
         ("map_at", c_i32), ("position_at", c_i32), ("merges_at", c_i32), ("tiles_at", c_i32), ("workers_at", c_i32),
         ("segments_at", c_i32),
     ]

@@ -133,9 +133,10 @@ size_t workspace_bytes_of(const gk_prefill_params* p, const gk_shared_prefix_lis
 }  // namespace
 
 int shared_prefix_list_build(const int32_t* run_first_row, const int32_t* run_rows, const int32_t* run_pos,
-                             const int32_t* run_group, const int32_t* run_request, int32_t runs, const int32_t* group_prefix, int32_t groups,
-                             int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t sliding_window,
-                             int32_t* words, int64_t capacity, gk_shared_prefix_list* list) {
+                             const int32_t* run_group, const int32_t* run_request, int32_t runs,
+                             const int32_t* group_prefix, int32_t groups, int32_t q_heads, int32_t kv_heads,
+                             int32_t head_dim, int32_t sliding_window, int32_t* words, int64_t capacity,
+                             gk_shared_prefix_list* list) {
   const char* const name = "gk_shared_prefix_list_build";
   const auto bad = [&](const char* what) { return fail(GK_ERR_INVALID_ARGUMENT, std::string(name) + ": " + what); };
   if (!list || list->struct_size != sizeof(gk_shared_prefix_list))
@@ -159,7 +160,7 @@ int shared_prefix_list_build(const int32_t* run_first_row, const int32_t* run_ro
   if (rows > 65535) return bad("too many rows");
   try {
     std::vector<SharedRun> in(runs);
-    for (int32_t i = 0; i < runs; ++i) 
+    for (int32_t i = 0; i < runs; ++i)
       in[i] = {run_first_row[i], run_rows[i], run_pos[i], run_group[i], run_request ? run_request[i] : -1};
     const SharedPlan plan =
         shared_plan(in.data(), runs, group_prefix, q_heads / kv_heads, kv_heads, head_dim, sliding_window, device_cus());
@@ -176,6 +177,10 @@ int shared_prefix_list_build(const int32_t* run_first_row, const int32_t* run_ro
     list->worker_groups = plan.worker_groups;
     list->part_cols = plan.cols;
     list->can_store = plan.stores;
+    list->q_heads = q_heads;
+    list->kv_heads = kv_heads;
+    list->head_dim = head_dim;
+    list->sliding_window = sliding_window > 0 ? sliding_window : -1;
     list->map_at = reserve(list->rows);
     list->position_at = reserve(list->rows);
     list->merges_at = reserve(int64_t{kSharedMergeWords} * list->rows);
@@ -208,6 +213,9 @@ int shared_prefix_attention(const gk_prefill_params* p, const gk_shared_prefix_l
   if (int rc = check_prefill(p, true, name)) return rc;
   if (!list || list->struct_size != sizeof(gk_shared_prefix_list))
     return fail(GK_ERR_INVALID_ARGUMENT, std::string(name) + ": struct_size does not match this library's gk_shared_prefix_list");
+  if (list->q_heads != p->q_heads || list->kv_heads != p->kv_heads || list->head_dim != p->head_dim ||
+      list->sliding_window != (p->sliding_window > 0 ? p->sliding_window : -1))
+    return fail(GK_ERR_INVALID_ARGUMENT, std::string(name) + ": the list was built for other heads or another window");
   if (list->rows < 0 || list->rows > 65535 || list->tile_count < 0 || list->workers < 0 || list->worker_groups < 0 ||
       list->worker_groups != (list->workers + kSharedWaves - 1) / kSharedWaves || list->part_cols < 0 ||
       list->part_cols > INT32_MAX)
@@ -288,8 +296,8 @@ extern "C" int gk_shared_prefix_list_build(const int32_t* run_first_row, const i
                                            int32_t kv_heads, int32_t head_dim, int32_t sliding_window, int32_t* words,
                                            int64_t capacity, gk_shared_prefix_list* list) {
   gk::clear_error();
-  return gk::shared_prefix_list_build(run_first_row, run_rows, run_pos, run_group, run_request, runs, group_prefix, groups, q_heads,
-                                      kv_heads, head_dim, sliding_window, words, capacity, list);
+  return gk::shared_prefix_list_build(run_first_row, run_rows, run_pos, run_group, run_request, runs, group_prefix,
+                                      groups, q_heads, kv_heads, head_dim, sliding_window, words, capacity, list);
 }
 
 extern "C" size_t gk_shared_prefix_workspace_bytes(const gk_prefill_params* params, const gk_shared_prefix_list* list) {

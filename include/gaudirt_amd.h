@@ -228,7 +228,10 @@ int gk_paged_prefill_listed(const gk_prefill_params* params, const gk_prefill_li
  *   score + slopes[head] * (key position - query position)
  * after the scale and the optional softcap; slopes: fp32 [q_heads] on the
  * device, finite. A row's own key has no bias; with a positive slope farther
- * keys weigh less. No counterpart in the reference.
+ * keys weigh less, and slopes above 2^20 (whose next key already weighs zero)
+ * count as 2^20. Negative slopes, under which farther keys weigh more, hold while
+ * |slope| * context stays below 2^16: beyond it a score's own digits drown in
+ * its bias. No counterpart in the reference.
  * ------------------------------------------------------------------------- */
 size_t gk_paged_decode_alibi_workspace_bytes(const gk_decode_params* params);
 int gk_paged_decode_alibi(const gk_decode_params* params, const float* slopes, void* workspace,
@@ -251,7 +254,7 @@ int gk_paged_prefill_alibi(const gk_prefill_params* params, const gk_prefill_lis
  * No counterpart in the reference, which attends every row by itself.
  *
  * gk_shared_prefix_list_build (host only) plans the work of host-known lengths:
- * it fills `list` but for its two pointers and writes word_count words
+ * it fills `list` but for its pointers and new_kv_row_stride and writes word_count words
  * (GK_ERR_WORKSPACE, with word_count set, when capacity is smaller). run_request:
  * block-table row of each run, or NULL where only the device knows them. The caller
  * copies the words to the device, 16-byte aligned, and sets words to the copy
@@ -261,8 +264,11 @@ int gk_paged_prefill_alibi(const gk_prefill_params* params, const gk_prefill_lis
  * new_value hold their rows (batch rows, as gk_kv_store takes them), which the
  * call attends and stores at the slots of their positions.
  * gk_shared_prefix_attention does not read seq_*, seqs and max_rows of its
- * gk_prefill_params and writes the list's rows only; its sliding_window is the
- * list's. A GQA group of at most 128; at most 65535 rows.
+ * gk_prefill_params and writes the list's rows only; its heads and sliding_window
+ * are the list's (checked). A GQA group of at most 128; at most 65535 rows. Rows
+ * that share a tile share its keys' values, as in gk_paged_prefill: an infinite
+ * or NaN value at a token that one row of a run or group sees reaches the others'
+ * outputs, also of rows before it.
  * ------------------------------------------------------------------------- */
 typedef struct gk_shared_prefix_list {
   size_t struct_size;          /* sizeof(gk_shared_prefix_list) as the caller was built; checked */
@@ -273,13 +279,15 @@ typedef struct gk_shared_prefix_list {
   int64_t new_kv_row_stride;
   int64_t part_cols;           /* partial results of one kv head */
   int32_t rows, tile_count, workers, worker_groups, word_count, can_store;
+  int32_t q_heads, kv_heads, head_dim, sliding_window;  /* what it was built for; checked */
   int32_t map_at, position_at, merges_at, tiles_at, workers_at, segments_at;  /* sections of the words */
 } gk_shared_prefix_list;
 
 int gk_shared_prefix_list_build(const int32_t* run_first_row, const int32_t* run_rows, const int32_t* run_pos,
-                                const int32_t* run_group, const int32_t* run_request, int32_t runs, const int32_t* group_prefix, int32_t groups,
-                                int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t sliding_window,
-                                int32_t* words, int64_t capacity, gk_shared_prefix_list* list);
+                                const int32_t* run_group, const int32_t* run_request, int32_t runs,
+                                const int32_t* group_prefix, int32_t groups, int32_t q_heads, int32_t kv_heads,
+                                int32_t head_dim, int32_t sliding_window, int32_t* words, int64_t capacity,
+                                gk_shared_prefix_list* list);
 size_t gk_shared_prefix_workspace_bytes(const gk_prefill_params* params, const gk_shared_prefix_list* list);
 int gk_shared_prefix_attention(const gk_prefill_params* params, const gk_shared_prefix_list* list, void* workspace,
                                size_t workspace_bytes, hipStream_t stream);
@@ -467,7 +475,10 @@ int gk_block_tables(const int32_t* mapping, int32_t requests, int32_t context, i
  * ([0, slots / page_size)) is entered as -1, and its tokens get slot -1.
  *
  * The rows of a batch are distinct, and a parent holds the tokens before the
- * call (it may itself get more in it). Status 0, or the first sequence in batch
+ * call (it may itself get more in it, but not start from a parent). The outputs
+ * overlap no input: counts lies apart from free_head, out_lengths from prefixes
+ * and lengths (checked), since workgroups read the inputs while others write.
+ * Status 0, or the first sequence in batch
  * order that cannot be served, and why; nothing but rows of slot -1, unchanged
  * out_lengths and counts {0, *free_head, ...} is then written:
  *   1 its row, or its parent, outside [0, requests)

@@ -178,6 +178,20 @@ def test_free_list_head_and_bad_pages():
     Step(15, [(0, 40, -1)], free=[8, 9, 10], slots=9 * 16).check()                # page 8 is the last one
 
 
+@pytest.mark.parametrize("seqs", [2, 1100])
+@pytest.mark.parametrize("page", [-1, 1 << 20, (1 << 28) + 1])
+def test_cached_pages_outside_the_pool(seqs, page):
+    # A table row that was never filled: the tokens that continue such a page get no slot, whatever their page's entry is.
+    put = lambda v, t=torch.int32: torch.tensor(v, device="cuda", dtype=t)  # noqa: E731
+    tables = torch.full((seqs, 4), page, device="cuda", dtype=torch.int32)
+    locations, requests, positions, lengths, counts = torch.ops.gaudirt.extend_block_tables(
+        tables, None, put(list(range(seqs))), put([5] * seqs), put([3] + [0] * (seqs - 2) + [12]), put([1, 2], torch.int64),
+        None, None, 16, 64, 15)
+    assert counts.tolist() == [15, 1, 0, -1]
+    assert locations.tolist() == [-1] * 14 + [16] and positions.tolist() == [5, 6, 7] + list(range(5, 17))
+    assert tables[-1].tolist() == [page, 1, page, page]
+
+
 @pytest.mark.parametrize("step,rows,status", [
     (dict(seqs=[(0, 3, -1), (500, 13, -1)]), None, 2), (dict(seqs=[(0, 3, -1), (513, 0, -1)]), None, 2),
     (dict(seqs=[(-1, 3, -1)]), None, 2), (dict(seqs=[(5, 1, -1), (5, -1, -1)]), 9, 2),

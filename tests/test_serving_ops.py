@@ -74,3 +74,18 @@ def test_extend_refuses(change, message):
 
 def test_extend_refuses_null():
     assert capi.load().gk_extend_block_tables(None, None) == capi.GK_ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("out,inputs,offset,length", [
+    ("counts", "free_head", 12, 4), ("counts", "free_head", 0, 4), ("out_lengths", "prefixes", 0, 8),
+    ("out_lengths", "prefixes", -28, 8), ("out_lengths", "lengths", 12, 4),
+])
+def test_extend_refuses_outputs_over_inputs(out, inputs, offset, length):
+    p = extend_params()
+    for i, (field, kind) in enumerate(p._fields_):
+        if kind is ctypes.c_void_p:
+            setattr(p, field, (1 << 20) + (i << 12))
+    p.lengths_int64 = length == 8
+    setattr(p, inputs, getattr(p, out) + offset)
+    assert capi.load().gk_extend_block_tables(ctypes.byref(p), None) == capi.GK_ERR_INVALID_ARGUMENT
+    assert "overlap" in capi.load().gk_last_error().decode()

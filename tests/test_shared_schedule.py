@@ -104,3 +104,13 @@ def test_attention_refuses(change, code, message):
     assert lib.gk_shared_prefix_attention(ctypes.byref(p), ctypes.byref(lst), ctypes.c_void_p(1 << 20), short,
                                           None) == code
     assert message in lib.gk_last_error().decode()
+
+
+@pytest.mark.parametrize("field,value", [("q_heads", 64), ("kv_heads", 16), ("head_dim", 64), ("sliding_window", 100)])
+def test_attention_refuses_another_geometry(field, value):
+    p, lst = attention_args()
+    setattr(p, field, value)
+    p.q_row_stride = p.out_row_stride = 64 * 128
+    assert capi.load().gk_shared_prefix_attention(ctypes.byref(p), ctypes.byref(lst), ctypes.c_void_p(1 << 20), 1 << 40,
+                                                  None) == capi.GK_ERR_INVALID_ARGUMENT
+    assert "built for other heads" in capi.load().gk_last_error().decode()
