@@ -16,6 +16,13 @@
 //     (shared_schedule.hpp) gives the workers as many CUs as their bytes need
 //     while the other CUs multiply.
 //  2. the merge, one workgroup per (row, head).
+// Measured, whole call, against every row by itself (us): 64 rows of 32 q / 8 kv
+// heads behind 4096 shared tokens, 32 to 1023 of their own (head_dim 128, 164 MB
+// once each) 36.8 / 175, of which the first launch ~30 and the merge 4.0-4.6; 256
+// rows behind 32000 (515 MB, 136 GFLOP) 171-176 / 4110, tiles at 1.2 PFLOP/s on 24
+// of a kv head's 32 CUs beside workers on the other eight, merge 7.1; 48 rows of
+// 16 q / 8 kv heads at head_dim 256 with a window (753 MB) 135 / 256, 5.6 TB/s
+// over the call, 6.5 in the steady part.
 #include "shared_worker.hpp"
 
 #include <cstring>
@@ -278,11 +285,18 @@ int shared_prefix_attention(const gk_prefill_params* p, const gk_shared_prefix_l
   const dim3 mgrid((unsigned)p->q_heads, (unsigned)list->rows);
   const auto merge = [&](auto waves) {
     constexpr int W = decltype(waves)::value;
-    if (p->head_dim == 64) shared_merge_kernel<64, W><<<mgrid, W * 64, 0, stream>>>(m);
+    if (p->head_dim == 64) shared_merge_kernel<64, W == 8 ? 4 : W><<<mgrid, (W == 8 ? 4 : W) * 64, 0, stream>>>(m);
     else if (p->head_dim == 128) shared_merge_kernel<128, W><<<mgrid, W * 64, 0, stream>>>(m);
     else shared_merge_kernel<256, W><<<mgrid, W * 64, 0, stream>>>(m);
   };
-  if ((int64_t)list->rows * p->q_heads <= 512) merge(std::integral_constant<int, 4>{});
+  // Few (row, head) pairs have many parts each and leave CUs idle: more waves take a pair's parts side by side. Many
+  // pairs fill the GPU by themselves. One / four / eight waves (us): head_dim 128, 32 pairs 21.4 / 7.0 / 5.2, 256 pairs
+  // 13.4 / 5.7 / 5.5, 512 4.2 / 3.9 / 4.0, 1024 5.6 / 5.2 / 5.2, 2048 6.0 / 6.0 / 7.3, 8192 6.4 / 10.0 / 15.6; head_dim
+  // 256, 128 pairs 30.3 / 10.3 / 7.0, 1024 6.4 / 5.9 / 5.6, 2048 5.7 / 5.9 / 7.4; head_dim 64, where four waves hold 16
+  // parts already, 56 pairs 11.4 / 4.7 / 5.0, 896 4.0 / 4.0 / 5.3, 1792 4.3 / 4.8 / 7.1.
+  const int64_t pairs = (int64_t)list->rows * p->q_heads;
+  if (pairs <= 512) merge(std::integral_constant<int, 8>{});
+  else if (pairs <= 1024) merge(std::integral_constant<int, 4>{});
   else merge(std::integral_constant<int, 1>{});
   return hip_status(hipGetLastError(), "gk_shared_prefix_attention merge launch");
 }
