@@ -9,6 +9,11 @@ for it (python/gaudirt/__init__.py, src/bridge/generic_private_use1.cpp:430-540)
   ``torch.classes.gaudirt.PagedMetadata`` are registered by the HIP extension
   ``gaudirt_amd._C``, together with ``rotary_paged_attn`` (rotary embedding
   fused into the attention's KV store; no counterpart in the reference);
+- so are three serving operators without a counterpart: ``shared_prefix_attn``
+  (groups of rows behind a shared prefix, its keys read once a group),
+  ``paged_attn_alibi`` (a distance bias with a slope per head) and
+  ``extend_block_tables`` (tables, map and slots of a scheduler step from lengths
+  on the device);
 - ``allocate_paged_kv(layers, slots, kv_heads, head_dim)`` returns a zeroed
   head-major bf16 pool ``[layers, 2, kv_heads, slots, head_dim]`` from the
   stream-ordered block allocator, and ``kv_pool_views(pool, layer)`` its

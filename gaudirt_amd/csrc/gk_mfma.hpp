@@ -45,8 +45,8 @@ __device__ __forceinline__ float soft_cap(float x, float cap) {
 //  kScoreCap      cap * tanh(q . k * scale / cap), in log2 units;
 //  kScoreBias     plain plus slope_head * (key position - query position), in
 //                 the raw product's units so that the scale still rides in the
-//                 exponent: decode starts its accumulators from it, prefill adds
-//                 it where the maxima are taken;
+//                 exponent: decode starts its accumulators from it, prefill too
+//                 or adds it where the maxima are taken;
 //  kScoreCapBias  kScoreCap plus slope_head * distance.
 constexpr int kScorePlain = 0, kScoreCap = 1, kScoreBias = 2, kScoreCapBias = 3;
 constexpr bool score_capped(int score) { return score == kScoreCap || score == kScoreCapBias; }

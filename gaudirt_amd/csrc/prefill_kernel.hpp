@@ -484,6 +484,21 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
   f32x4_t sc[kKG][kNT];
   bf16x8_t pa[kKH][kNT];
 
+  // A distance bias's part inside the step (slope times the key's offset): the
+  // scores' accumulators start from it where the registers hold it, else the
+  // softmax adds it, one instruction a score. Starting / adding (us): head_dim 64,
+  // 8 x 512 rows on 2048 tokens, 32 heads 139.8 / 144.4, 2 x 1000 on 16000 453.6 /
+  // 466.8; head_dim 256, 16 heads 196.1 / 197.8, 581.7 / 585.0; head_dim 128, where
+  // starting spills 38 registers, 266 / 175.
+  constexpr bool kBiasFirst = SCORE == kScoreBias && D != 128;
+  [[maybe_unused]] f32x4_t inside[kKG][kNT];
+  if constexpr (kBiasFirst) {
+#pragma unroll
+    for (int h = 0; h < kKG; ++h)
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) inside[h][nt] = bias4(slope[nt], 0.f, h);
+  }
+
   // S^T = K.Q^T into sc: lane (q, c16) gets qrow c16 (+16 nt), keys tb + 16h + 4q + r.
   auto scores = [&](const char* kt) __attribute__((always_inline)) {
 #pragma unroll
@@ -495,7 +510,8 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
         kr[c] = *reinterpret_cast<const bf16x8_t*>(kt + tt * (2 * D) + (((4 * c + q) ^ swz(tt, D / 8)) << 4));
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
-        sc[h][nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        if constexpr (kBiasFirst) sc[h][nt] = inside[h][nt];
+        else sc[h][nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < S::NC; ++c) sc[h][nt] = mfma32(kr[c], qb[nt][c], sc[h][nt]);
       }
@@ -542,10 +558,10 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
   // scores (scale > 0), and p = exp2(fma(s, scale, -max)).
   auto softmax = [&](int tb) __attribute__((always_inline)) {
     const bool full = tb + kKeys - 1 <= wave_pos_min && tb >= wave_left_max;
-    // With a distance bias the scores get its part inside the step (slope times
-    // the key's offset) here, one instruction each; the rest, the same for all of
-    // a lane's keys, joins the maximum and the exponent's base.
-    if constexpr (!LOG2 && SCORE != kScoreBias) mfma_results_ready(sc);
+    // With a distance bias the scores hold its part inside the step from the start
+    // or get it here; the rest, the same for all of a lane's keys, joins the maximum
+    // and the exponent's base.
+    if constexpr (!LOG2 && (SCORE != kScoreBias || kBiasFirst)) mfma_results_ready(sc);
     // Mask, and each tile's row maximum over this lane's 4 kKG scores.
     float mx[kNT];
     [[maybe_unused]] float bias0[kNT];
@@ -564,10 +580,12 @@ __global__ __launch_bounds__(kPrefillWaves * 64, 1) void prefill_kernel(Args a) 
       }
       if constexpr (SCORE == kScoreBias) {
         bias0[nt] = slope[nt] * (float)(tb + 4 * q - qpos[nt]);
+        if constexpr (!kBiasFirst) {
 #pragma unroll
-        for (int h = 0; h < kKG; ++h)
+          for (int h = 0; h < kKG; ++h)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sc[h][nt][r] = __builtin_fmaf(slope[nt], (float)(16 * h + r), sc[h][nt][r]);
+            for (int r = 0; r < 4; ++r) sc[h][nt][r] = __builtin_fmaf(slope[nt], (float)(16 * h + r), sc[h][nt][r]);
+        }
       }
       if (!full) {
 #pragma unroll
