@@ -6,10 +6,10 @@
 // Rows come in groups whose rows hold the same slots for the group's first
 // `prefix` tokens. The group's columns, (row, head) pairs of one kv head, attend
 // those keys together: in tiles of up to prefill_tile_qrows columns (eight waves
-// on one K/V tile in LDS) or, where they are few, as one wave's columns. Behind
-// the prefix every run of rows (consecutive positions of one request) attends
-// its own keys. Both kinds of work are cut along their keys; each piece leaves
-// an unnormalised partial, and a second launch joins a row's partials.
+// on one K/V tile in LDS) or, where columns are few and keys many, as one wave's
+// columns. Behind the prefix every run of rows (consecutive positions of one
+// request) attends its own keys. Both kinds of work are cut along their keys; each
+// piece leaves an unnormalised partial, and a second launch joins a row's partials.
 #pragma once
 
 #include <algorithm>
@@ -107,18 +107,34 @@ inline SharedPlan shared_plan(const SharedRun* runs, int count, const int32_t* g
   SharedPlan plan;
   const int tile_cols = prefill_tile_qrows(head_dim), tile_rows = tile_cols / group;
   const int step_keys = shared_step_keys(head_dim), key_tile = shared_tile_keys(head_dim);
-  const int columns = shared_columns(head_dim);
+  const int columns = shared_columns(head_dim), slots = std::max(1, cus / kv_heads);
+  // Prefixes of few columns, in keys a CU: what decides who attends them. Workers stream at HBM's rate, but each
+  // leaves a partial of every column; a tile's workgroup leaves one and streams at two thirds of the rate. Whole call,
+  // tile / worker (us), head_dim 128: 375 keys a CU, 8 columns 17.1 / 19.4, 12 17.7 / 23.2; 1000 keys, 8 columns 28.6
+  // / 29.6, 16 29.7 / 33.5, 32 32.7 / 42.3; 750 keys, 4 columns 33.8 / 26.6; 1500 keys, 2 columns 50.2 / 40.1, 3000
+  // keys, 4 columns 120 / 72, 16 columns 124 / 84. head_dim 256: 375 keys, 2 columns 23.0 / 25.8, 16 23.7 / 36.4;
+  // 1500, 6 columns 92 / 81. head_dim 64: 375 keys, 21 columns 15.2 / 17.5; 3000, 7 columns 86 / 41.
+  int64_t few_keys = 0;
+  for (int i = 0; i < count;) {
+    const int g = runs[i].group;
+    int rows = 0, low = INT32_MAX;
+    for (; i < count && runs[i].group == g; ++i) {
+      rows += runs[i].rows;
+      low = std::min(low, runs[i].pos);
+    }
+    if (rows % tile_rows && rows % tile_rows * group <= columns)
+      few_keys += std::max(0, group_prefix[g] - (window > 0 ? std::max(0, low - window + 1) : 0));
+  }
+  const int64_t few_a_cu = few_keys / slots;
+  const int prefix_columns = few_a_cu <= 512 ? 0 : few_a_cu <= 1024 ? columns / 4 : columns;  // of a worker, at most
   std::vector<SharedWork> wide, narrow;
   std::vector<int32_t> row_request;  // of compact rows
   const auto add = [&](int first, int rows, int lo, int hi, int run) {
-    // A tile takes what has more columns than a worker holds (own keys: than two
-    // hold, which streams them twice at most). Tile / worker, whole call (us): 32 q /
-    // 8 kv heads, 120 columns on 2300 prefix keys 19.7 / 24.5; 8 q / 8 kv heads, 30
-    // columns on 8000 19.0 / 20.5, within a call's spread of the batch.
+    // Own keys are a worker's up to the columns of two, which streams them twice at most.
     if (lo >= hi) return;
     const bool own = run >= 0;
     SharedWork w{first, rows, lo, hi, run, 0, 0};
-    const bool tile = group > columns || rows * group > (own ? 2 * columns : columns);
+    const bool tile = group > columns || rows * group > (own ? 2 * columns : prefix_columns);
     if (tile) {
       w.start = lo / step_keys * step_keys;
       w.units = (hi - w.start + step_keys - 1) / step_keys;
@@ -183,7 +199,6 @@ inline SharedPlan shared_plan(const SharedRun* runs, int count, const int32_t* g
   // How many of a kv head's CUs take workers: the number with which both kinds
   // of work, side by side, end soonest.
   const SharedCost cost = shared_cost(head_dim);
-  const int slots = std::max(1, cus / kv_heads);
   int64_t key_tiles = 0;
   for (const auto& w : narrow) key_tiles += w.units;
   int best = narrow.empty() ? 0 : slots;

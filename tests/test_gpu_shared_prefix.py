@@ -153,6 +153,20 @@ def test_long_prefix():
     check(Batch(14, decode(1, 5, 500), [20000], heads=(14, 2, 64)))
 
 
+# Groups of few columns, (rows of a group) x (heads a kv head), on prefixes of more than 512, or 1024, keys a CU of a kv
+# head: all in tiles below, in waves of their own above, those of more than a quarter of a wave's columns between.
+@pytest.mark.parametrize("heads,groups,rows,prefix", [
+    ((32, 32, 64), 6, 3, 1600), ((32, 32, 64), 6, 20, 1600), ((64, 32, 64), 6, 16, 1600), ((64, 16, 128), 6, 4, 3001),
+    ((64, 16, 128), 6, 7, 3001), ((32, 16, 256), 6, 1, 3001), ((32, 16, 256), 6, 8, 3001),
+    ((32, 32, 64), 4, 5, 1600), ((64, 16, 128), 4, 3, 2600), ((32, 16, 256), 4, 5, 2600),
+])
+def test_few_columns_on_many_keys(heads, groups, rows, prefix):
+    b = Batch(20, decode(groups, rows, 60), [prefix - 16 * g for g in range(groups)], heads=heads)
+    check(b)
+    check(b, softcap=30.0, window=1500)
+    check(b, window=prefix - 40)
+
+
 def test_extreme_values():
     # Scores of a few thousand, values near bf16's largest: weights of 0 and 1, no infinity on the way.
     b = Batch(15, decode(2, 9, 200), [300, 128], value_scale=1e37)
